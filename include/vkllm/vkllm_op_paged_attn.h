@@ -1,0 +1,40 @@
+/* VKLLM_OP_PAGED_ATTN: attention of one new token of each sequence of a batch over a paged cache. No counterpart in the
+ * reference.
+ *
+ * The tensor and srcs[0], the queries, are [1, B, H, head_dim] of any strides; srcs[1] is the cache (VKLLM_OP_UPDATE_PAGES,
+ * [pages, 2 * KV, page_rows, head_dim], packed, page_rows a multiple of 16, H a multiple of KV: query head h reads key
+ * head h / (H / KV)), all fp16 or all fp32; srcs[2] is the page table (VKLLM_OP_PAGE_TABLE, uint32 [1, 1, B, 1 + P], B <= 4096).
+ * Row b is the last token of its sequence, whose keys and values the cache holds already: over positions j < length
+ * out = sum_j softmax_j(scale * q . k_j) v_j, with q rotated to position length - 1 (unless rope_base is 0). Softmax and
+ * sums are in 32 bits, and the result is rounded once. A row of length 0 gives zeros; lengths end at P * page_rows, and
+ * positions on pages that the cache does not have count as absent. Rows of the cache past a sequence's end
+ * are never used, whatever they hold.
+ * _init sets up the context's workspace: code that captures _run into a hipGraph calls _init and _run once before. */
+#ifndef VKLLM_OP_PAGED_ATTN_H
+#define VKLLM_OP_PAGED_ATTN_H
+#include <stdbool.h>
+#include <stdint.h>
+#include "vkllm_commands.h"
+#include "vkllm_context.h"
+#include "vkllm_tensor.h"
+#ifdef __cplusplus
+extern "C" {
+#endif
+
+struct vkllm_op_paged_attn_params
+{
+    float scale;
+    float rope_base; /* as in vkllm_op_update_pages_params */
+    bool neox_style;
+};
+extern vkllm_err_t vkllm_op_paged_attn_init(struct vkllm_context *context, struct vkllm_commands *commands,
+                                    struct vkllm_tensor *tensor);
+extern vkllm_err_t vkllm_op_paged_attn_run(struct vkllm_context *context, struct vkllm_commands *commands,
+                                   struct vkllm_tensor *tensor);
+extern vkllm_err_t vkllm_op_paged_attn_post_run(struct vkllm_context *context, struct vkllm_commands *commands,
+                                        struct vkllm_tensor *tensor);
+
+#ifdef __cplusplus
+}
+#endif
+#endif

@@ -93,7 +93,9 @@ extern "C" const char *vkllm_op_s(const vkllm_op_t op)
     static const char *names[] = {"VKLLM_OP_NONE",      "VKLLM_OP_COPY",    "VKLLM_OP_BIN",
                                   "VKLLM_OP_EMBEDDING", "VKLLM_OP_RMSNORM", "VKLLM_OP_MATMUL",
                                   "VKLLM_OP_ROPE",      "VKLLM_OP_SOFTMAX", "VKLLM_OP_FFN_UP_AND_GATE",
-                                  "VKLLM_OP_UPDATE_ROWS", "VKLLM_OP_ARG_MAX", "VKLLM_OP_REF"};
+                                  "VKLLM_OP_UPDATE_ROWS", "VKLLM_OP_ARG_MAX", "VKLLM_OP_REF",
+                                  "VKLLM_OP_PAGE_TABLE", "VKLLM_OP_SLOT_MAP", "VKLLM_OP_UPDATE_PAGES",
+                                  "VKLLM_OP_PAGED_ATTN", "VKLLM_OP_ADJUST_LOGITS"};
     if ((int)op < 0 || (int)op >= (int)(sizeof(names) / sizeof(names[0])))
         return "VKLLM_OP_COUNTS";
     return names[op];
@@ -203,7 +205,8 @@ static const char *kernel_names[KID_COUNT] = {
     "rope",          "softmax",       "ffn_up_and_gate", "update_rows",   "arg_max",       "fused_embed",
     "fused_qkv_rope", "fused_attn_scores", "fused_attn_pv", "fused_o_resid", "fused_gateup", "fused_down_resid",
     "fused_logits",  "fused_argmax",  "fused_rmsnorm",   "fused_gemm",    "fused_rope_kv", "fused_attn_prefill",
-    "fused_swiglu",   "fused_attn_small", "fused_attn_o",    "fused_attn_long"};
+    "fused_swiglu",   "fused_attn_small", "fused_attn_o",    "fused_attn_long",
+    "page_table",    "slot_map",      "update_pages",    "paged_attn",    "adjust_logits"};
 
 vkllm_pipeline *pipeline_of(vkllm_context *ctx, KernelId id)
 {

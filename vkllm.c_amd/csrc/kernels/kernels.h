@@ -44,6 +44,49 @@ hipError_t launch_update_rows(hipStream_t st, const TView &src, const TView &cac
 hipError_t launch_arg_max(hipStream_t st, const TView &in, const TView &out);
 hipError_t launch_ffn_up_and_gate(hipStream_t st, const TView &x, const TView &wu, const TView &wg, const TView &out);
 
+// ---- batched generation over a paged cache ----
+constexpr uint32_t kPagedMaxRows = 4096;       // sequences of a batch (their prefix sums stand in LDS)
+constexpr uint32_t kPagedMaxPages = 512 << 10; // pages of a cache that PAGE_TABLE hands out (a bit each in LDS)
+constexpr uint32_t kPagedMaxHd = 256;
+
+// words [B, 1 + P] of a page table, `stride` words from row to row
+struct PageTableView
+{
+    uint32_t *p;
+    uint32_t B, P, stride;
+};
+// want [B] with element stride want_s; old: the table so far, or nullptr to bring `out` up to date in place
+hipError_t launch_page_table(hipStream_t st, const PageTableView &out, const uint32_t *old, uint32_t old_stride,
+                             const uint32_t *want, uint32_t want_s, uint32_t page_rows, uint32_t pages, int cu_count);
+// map [T] pairs (slot, position), packed
+hipError_t launch_slot_map(hipStream_t st, const PageTableView &table, const uint32_t *lengths, uint32_t lengths_s,
+                           const uint32_t *counts, uint32_t counts_s, uint32_t *map, uint32_t T, uint32_t page_rows);
+
+// RoPE by position * turns[w] full turns for pair w < head_dim / 2; the products are formed in 64 bits, since a far
+// position times a frequency has more turns than a 32-bit product keeps a fraction of
+struct PagedRope
+{
+    int style; // 0: none, 1: pairs (2w, 2w + 1), 2: pairs (w, w + head_dim / 2)
+    double turns[kPagedMaxHd / 2];
+};
+// cache [pages, 2 KV, R, hd] packed; k, v [1, T, KV, hd]; map [T] pairs with `map_s` words from token to token
+hipError_t launch_update_pages(hipStream_t st, const TView &cache, const TView &k, const TView &v, const uint32_t *map,
+                               uint32_t map_s, const PagedRope &rope);
+// q, out [1, B, H, hd]; `work` holds partial rows (work_elems floats)
+hipError_t launch_paged_attn(hipStream_t st, const TView &q, const TView &cache, const PageTableView &table,
+                             const TView &out, float scale, const PagedRope &rope, float *work, size_t work_elems,
+                             int cu_count);
+
+// words of a [B, ...] source, `stride` from row to row and `n` of them in a row; p == nullptr: not given
+struct WordRows
+{
+    const uint32_t *p;
+    uint32_t stride, n;
+};
+// x, out [1, 1, B, V], contiguous in V
+hipError_t launch_adjust_logits(hipStream_t st, const TView &x, const TView &out, const WordRows &history,
+                                const WordRows &rules, const WordRows &mask);
+
 // ---- fused LLaMA-2 token step ----
 // Device-resident step parameters, read by the kernels so a captured decode graph replays for any position.
 struct Step

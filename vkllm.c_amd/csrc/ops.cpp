@@ -4,65 +4,22 @@
 #include <cmath>
 #include <cstring>
 
-#include "runtime.h"
+#include "ops_common.h"
+#include "vkllm/vkllm_op_adjust_logits.h"
 #include "vkllm/vkllm_op_arg_max.h"
 #include "vkllm/vkllm_op_bin.h"
 #include "vkllm/vkllm_op_copy.h"
 #include "vkllm/vkllm_op_embedding.h"
 #include "vkllm/vkllm_op_ffn_up_and_gate.h"
 #include "vkllm/vkllm_op_matmul.h"
+#include "vkllm/vkllm_op_page_table.h"
+#include "vkllm/vkllm_op_paged_attn.h"
 #include "vkllm/vkllm_op_rmsnorm.h"
 #include "vkllm/vkllm_op_rope.h"
+#include "vkllm/vkllm_op_slot_map.h"
 #include "vkllm/vkllm_op_softmax.h"
+#include "vkllm/vkllm_op_update_pages.h"
 #include "vkllm/vkllm_op_update_rows.h"
-
-static bool same_shape(const vkllm_tensor *a, const vkllm_tensor *b)
-{
-    return a->shapes[0] == b->shapes[0] && a->shapes[1] == b->shapes[1] && a->shapes[2] == b->shapes[2] &&
-           a->shapes[3] == b->shapes[3];
-}
-
-static bool is_float(vkllm_dtype_t d)
-{
-    return d == vkllm_dtype_float16 || d == vkllm_dtype_float32;
-}
-
-// Every view a kernel is given must stay inside its base allocation.
-static bool view_in_bounds(const vkllm_tensor *t)
-{
-    const vkllm_tensor *b = t;
-    while (b->data.is_ref && b->srcs[0])
-        b = b->srcs[0];
-    uint64_t last = 0;
-    for (int i = 0; i < 4; ++i)
-        last += (uint64_t)(t->shapes[i] - 1) * t->strides[i];
-    return last + dtype_bytes(t->dtype) <= b->bytes;
-}
-
-#define CHECK_VIEW(_t)                                                                                              \
-    do                                                                                                              \
-    {                                                                                                               \
-        if (!view_in_bounds(_t))                                                                                    \
-        {                                                                                                           \
-            log_error("tensor %s: view exceeds its allocation", (_t)->name);                                        \
-            return VKLLM_ERR_ARGS;                                                                                  \
-        }                                                                                                           \
-    } while (0)
-
-#define LAUNCH(_ctx, _kid, _call)                                                                                   \
-    do                                                                                                              \
-    {                                                                                                               \
-        hipError_t _e = timed((_ctx), pipeline_of((_ctx), (_kid)), [&]() { return (_call); });                     \
-        if (_e != hipSuccess)                                                                                       \
-            return hip_fail(_e, #_call, __FILE__, __LINE__);                                                        \
-    } while (0)
-
-#define NEED_DEV(_v)                                                                                                \
-    do                                                                                                              \
-    {                                                                                                               \
-        if (!(_v).p)                                                                                                \
-            return VKLLM_ERR_ALLOC;                                                                                 \
-    } while (0)
 
 // =============================================================================================================
 // COPY: src/core/vkllm_op_copy.c:11-30 (init), :32-122 (run)
@@ -320,9 +277,9 @@ static hipError_t launch_op_gemv(vkllm_context *ctx, const vk::TView &a, const v
     return vk::launch_gemv(ctx->device->stream, vk::EPI_RAW, g, ctx->device->cu_count);
 }
 
-// 64 MB of split-K partials for the op's tile GEMM, made once per context (the kernels then split K only as far as
-// it fits); an allocation failure leaves K unsplit
-static vkllm_err_t op_gemm_workspace(vkllm_context *ctx, float **work, size_t *elems)
+// 64 MB for the tile GEMM's split-K partials and the paged attention's partial rows, made once per context and used in
+// stream order (the kernels split only as far as it fits); an allocation failure leaves it empty
+vkllm_err_t op_workspace(vkllm_context *ctx, float **work, size_t *elems)
 {
     vkllm_gpu_device *dev = ctx->device;
     if (!dev->op_work)
@@ -400,7 +357,7 @@ extern "C" vkllm_err_t vkllm_op_matmul_run(struct vkllm_context *context, struct
     {
         float *work = nullptr;
         size_t work_elems = 0;
-        _CHECK(op_gemm_workspace(context, &work, &work_elems));
+        _CHECK(op_workspace(context, &work, &work_elems));
         LAUNCH(context, kid,
                vk::launch_gemm(context->device->stream, p.act ? vk::GEMM_SILU_HI : vk::GEMM_PLAIN,
                                (const uint16_t *)av.p, (const uint16_t *)bv.p, (uint16_t *)out.p, M, N, K, out.s[2], 0,
@@ -716,7 +673,7 @@ extern "C" vkllm_err_t vkllm_op_ffn_up_and_gate_run(struct vkllm_context *contex
     {
         float *work = nullptr;
         size_t work_elems = 0;
-        _CHECK(op_gemm_workspace(context, &work, &work_elems));
+        _CHECK(op_workspace(context, &work, &work_elems));
         LAUNCH(context, KID_FFN,
                vk::launch_gemm(context->device->stream, vk::GEMM_FFN, (const uint16_t *)x.p, (const uint16_t *)wu.p,
                                (uint16_t *)out.p, (uint32_t)rows, (2 * F + 63) / 64 * 64, K, F, F,
@@ -763,6 +720,16 @@ vkllm_err_t op_init(vkllm_context *ctx, vkllm_commands *cmds, vkllm_tensor *t)
         return vkllm_op_update_rows_init(ctx, cmds, t);
     case VKLLM_OP_ARG_MAX:
         return vkllm_op_arg_max_init(ctx, cmds, t);
+    case VKLLM_OP_PAGE_TABLE:
+        return vkllm_op_page_table_init(ctx, cmds, t);
+    case VKLLM_OP_SLOT_MAP:
+        return vkllm_op_slot_map_init(ctx, cmds, t);
+    case VKLLM_OP_UPDATE_PAGES:
+        return vkllm_op_update_pages_init(ctx, cmds, t);
+    case VKLLM_OP_PAGED_ATTN:
+        return vkllm_op_paged_attn_init(ctx, cmds, t);
+    case VKLLM_OP_ADJUST_LOGITS:
+        return vkllm_op_adjust_logits_init(ctx, cmds, t);
     default:
         log_error("Unknown operation type: %d", (int)t->op);
         return VKLLM_ERR_ARGS;
@@ -796,6 +763,16 @@ vkllm_err_t op_run(vkllm_context *ctx, vkllm_commands *cmds, vkllm_tensor *t)
         return vkllm_op_update_rows_run(ctx, cmds, t);
     case VKLLM_OP_ARG_MAX:
         return vkllm_op_arg_max_run(ctx, cmds, t);
+    case VKLLM_OP_PAGE_TABLE:
+        return vkllm_op_page_table_run(ctx, cmds, t);
+    case VKLLM_OP_SLOT_MAP:
+        return vkllm_op_slot_map_run(ctx, cmds, t);
+    case VKLLM_OP_UPDATE_PAGES:
+        return vkllm_op_update_pages_run(ctx, cmds, t);
+    case VKLLM_OP_PAGED_ATTN:
+        return vkllm_op_paged_attn_run(ctx, cmds, t);
+    case VKLLM_OP_ADJUST_LOGITS:
+        return vkllm_op_adjust_logits_run(ctx, cmds, t);
     default:
         log_error("Unknown operation type: %d", (int)t->op);
         return VKLLM_ERR_ARGS;

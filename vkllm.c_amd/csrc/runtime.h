@@ -55,6 +55,12 @@ enum KernelId
     KID_F_ATTN_SMALL,
     KID_F_ATTN_O,
     KID_F_ATTN_LONG,
+    // batched generation over a paged cache
+    KID_PAGE_TABLE,
+    KID_SLOT_MAP,
+    KID_UPDATE_PAGES,
+    KID_PAGED_ATTN,
+    KID_ADJUST_LOGITS,
     KID_COUNT
 };
 
@@ -93,7 +99,7 @@ struct vkllm_gpu_device
     vkllm_pipeline *timing_node = nullptr;
     std::vector<TimingRec> timing_pending;
     std::vector<hipEvent_t> event_pool;
-    // split-K partial tiles of the MATMUL op's matrix-core path, allocated at its first use (op_gemm_workspace)
+    // partial results of the operators that split their work, allocated at the first use (op_workspace)
     float *op_work = nullptr;
     size_t op_work_elems = 0;
 };

@@ -170,7 +170,7 @@ extern "C" vkllm_err_t vkllm_tensor_new(struct vkllm_context *context, const cha
         memset(t->data.host, 0, t->bytes);
     }
     // inputs, constants, caches and mapped tensors are backed now; other op outputs on first use
-    if (mapped || op == VKLLM_OP_NONE || op == VKLLM_OP_UPDATE_ROWS)
+    if (mapped || op == VKLLM_OP_NONE || op == VKLLM_OP_UPDATE_ROWS || op == VKLLM_OP_UPDATE_PAGES)
     {
         if (!tensor_dev(context, t))
         {

@@ -17,7 +17,9 @@ LIB_PATH = os.path.join(PKG, "build", "libvkllm.so")
 ERR_OK, ERR_ALLOC, ERR_VULKAN, ERR_DEV_NOT_FOUND, ERR_PIPELINE_NOT_FOUND, ERR_ARGS = 1, 2, 3, 4, 5, 6
 F32, F16, I8, U32 = 1, 2, 3, 4
 (OP_NONE, OP_COPY, OP_BIN, OP_EMBEDDING, OP_RMSNORM, OP_MATMUL, OP_ROPE, OP_SOFTMAX, OP_FFN_UP_AND_GATE,
- OP_UPDATE_ROWS, OP_ARG_MAX, OP_REF) = range(12)
+ OP_UPDATE_ROWS, OP_ARG_MAX, OP_REF, OP_PAGE_TABLE, OP_SLOT_MAP, OP_UPDATE_PAGES, OP_PAGED_ATTN,
+ OP_ADJUST_LOGITS) = range(17)
+NO_PAGE = NO_SLOT = 0xFFFFFFFF
 EXEC_FUSED, EXEC_NODES = 0, 1
 NP_DTYPE = {F32: np.float32, F16: np.float16, U32: np.uint32, I8: np.int8}
 DTYPE_OF = {np.dtype(np.float32): F32, np.dtype(np.float16): F16, np.dtype(np.uint32): U32, np.dtype(np.int8): I8}
@@ -57,7 +59,7 @@ class Graph(ctypes.Structure):
 
 class Stats(ctypes.Structure):
     _fields_ = [("tensor_alloc_counts", ctypes.c_int), ("tensor_free_counts", ctypes.c_int),
-                ("op_time_costs", ctypes.c_uint64 * 12), ("node_time_cost", ctypes.c_void_p)]
+                ("op_time_costs", ctypes.c_uint64 * 17), ("node_time_cost", ctypes.c_void_p)]
 
 
 class Context(ctypes.Structure):
@@ -141,8 +143,24 @@ class UpdateRowsParams(ctypes.Structure):
     _fields_ = [("offset_rows", ctypes.c_uint32)]
 
 
+class PageTableParams(ctypes.Structure):
+    _fields_ = [("page_rows", ctypes.c_uint32), ("pages", ctypes.c_uint32)]
+
+
+class SlotMapParams(ctypes.Structure):
+    _fields_ = [("page_rows", ctypes.c_uint32)]
+
+
+class UpdatePagesParams(ctypes.Structure):
+    _fields_ = [("rope_base", ctypes.c_float), ("neox_style", ctypes.c_bool)]
+
+
+class PagedAttnParams(ctypes.Structure):
+    _fields_ = [("scale", ctypes.c_float), ("rope_base", ctypes.c_float), ("neox_style", ctypes.c_bool)]
+
+
 OPS = ["copy", "bin", "embedding", "rmsnorm", "matmul", "rope", "softmax", "ffn_up_and_gate", "update_rows",
-       "arg_max"]
+       "arg_max", "page_table", "slot_map", "update_pages", "paged_attn", "adjust_logits"]
 
 _lib = None
 
