@@ -436,6 +436,8 @@ extern "C" void vkllm_context_free(struct vkllm_context *ctx)
             (void)hipEventDestroy(e);
         if (ctx->device->op_work)
             (void)hipFree(ctx->device->op_work);
+        if (ctx->device->paged_arrivals)
+            (void)hipFree(ctx->device->paged_arrivals);
         pool_release_all(ctx->device);
         node_pool_release(ctx->device);
         if (ctx->device->stream)

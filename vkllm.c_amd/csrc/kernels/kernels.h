@@ -72,10 +72,12 @@ struct PagedRope
 // cache [pages, 2 KV, R, hd] packed; k, v [1, T, KV, hd]; map [T] pairs with `map_s` words from token to token
 hipError_t launch_update_pages(hipStream_t st, const TView &cache, const TView &k, const TView &v, const uint32_t *map,
                                uint32_t map_s, const PagedRope &rope);
-// q, out [1, B, H, hd]; `work` holds partial rows (work_elems floats)
+// q, out [1, B, H, hd]; `work` holds partial rows (work_elems floats), `arrivals` kPagedArrivals counters that are zero
+// before the first launch and after each
+constexpr uint32_t kPagedMaxWorkgroups = 2048, kPagedArrivals = 4 * 2 * kPagedMaxWorkgroups;
 hipError_t launch_paged_attn(hipStream_t st, const TView &q, const TView &cache, const PageTableView &table,
                              const TView &out, float scale, const PagedRope &rope, float *work, size_t work_elems,
-                             int cu_count);
+                             uint32_t *arrivals, int cu_count);
 
 // words of a [B, ...] source, `stride` from row to row and `n` of them in a row; p == nullptr: not given
 struct WordRows

@@ -8,13 +8,17 @@
 // Work is split without knowing the lengths on the host: a unit is KT consecutive positions of one (sequence, key head),
 // all units of the batch are numbered in that order, and each of a fixed number of workgroups (as many as are resident)
 // takes an equal run of them. A (sequence, head) that ends up in several workgroups leaves partial sums in the workspace,
-// which a second kernel joins. A workgroup finds its units from prefix sums of the lengths, formed in LDS.
+// and whichever workgroup of a group of them is the last to arrive joins the group's, up a tree (join_up below). A workgroup
+// finds its units from prefix sums of the lengths, formed in LDS.
 //
 // Matrix cores do the products although 16 - G of their 16 columns are idle when G heads share a key head: they have 24
 // times the rate that the cache arrives at, and the layout spares the shuffles that dot products of single rows need.
 // Scores are K Q^T: a wave's 16 keys x 16 heads, of which lane l gets keys 4 (l / 16) + 0..3 of head l % 16. That is, with
 // the contraction numbered accordingly, the operand layout of V^T P^T, so probabilities stay in their lanes. V^T
 // wants several keys of one dim in a lane: a lane loads HDP / 16 dims of its 4 (8) keys and pairs them up by byte permutes.
+#include <algorithm>
+#include <type_traits>
+
 #include "device_common.h"
 #include "paged_common.h"
 
@@ -25,24 +29,53 @@ typedef _Float16 half8 __attribute__((ext_vector_type(8)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kHeadsPerTile = 16;
+// what starting and ending a (sequence, head) costs a workgroup, in units: 64 ragged rows of up to 8192 over 8 key heads
+// of 128 took 121 us with 0 and 117 with 1 (workgroups with many short rows had ended last)
+constexpr uint32_t kSegmentUnits = 1;
 constexpr float kNegInf = -INFINITY;
 
 struct PagedAttnArgs
 {
-    TView q, cache, out;
+    const void *q, *cache;
+    void *out;
+    uint32_t qs[3], os[3];            // element strides of q and out: sequence, head, dim
     PageTableView table;
-    float scale_log2;  // scale * log2(e)
-    uint32_t groups;   // tiles of 16 query heads per key head
-    uint32_t tile_heads; // min(16, heads per key head): rows of a partial result
-    float *parts;      // [workgroups][2] partial results
-    uint32_t *joins;   // [workgroups][4]: what each workgroup leaves to be joined
+    uint32_t pages, KV, G, hd;        // G query heads per key head
+    uint32_t page_tiles;              // tiles of 16 rows in a page
+    uint32_t page_bytes, head_bytes;  // of a page, and of one head in it
+    uint32_t groups;                  // tiles of 16 query heads per key head
+    uint32_t tile_heads;              // min(16, G): rows of a partial result
+    uint32_t div_magic, div_shift;    // t / page_tiles = t * div_magic >> div_shift for t < 2^28
+    float scale_log2;                 // scale * log2(e)
+    float *parts;                     // [workgroups][2] partial results
+    uint32_t *arrivals;               // [kJoinLevels][workgroups][2] counters, zero between launches
     PagedRope rope;
 };
 
-// a partial result: m [tile_heads], l [tile_heads], o [tile_heads][hd]
+// a partial result: o [tile_heads][hd], then (m, l) [tile_heads]
 __host__ __device__ __forceinline__ size_t part_floats(uint32_t tile_heads, uint32_t hd)
 {
     return (size_t)tile_heads * (hd + 2);
+}
+
+// Two floats of a partial result, written through to the level that all XCDs share and read from there: no workgroup needs
+// a device-wide fence, which would write back a whole L2
+__device__ __forceinline__ void put2(float *p, float x, float y)
+{
+    const uint64_t v = (uint64_t)__float_as_uint(y) << 32 | __float_as_uint(x);
+    __hip_atomic_store((uint64_t *)p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ float2 get2(const float *p)
+{
+    const uint64_t v = __hip_atomic_load((const uint64_t *)p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    return {__uint_as_float((uint32_t)v), __uint_as_float((uint32_t)(v >> 32))};
+}
+
+// A thread joins kJoinFan parts of two dims. Where a part has fewer than 256 pairs of dims, several threads share a pair.
+constexpr uint32_t kJoinFan = 8, kJoinLevels = 4; // 8^4 parts
+__device__ __forceinline__ uint32_t join_ways(uint32_t pairs)
+{
+    return pairs >= 256 ? 1 : min(8u, 256 / pairs);
 }
 
 template <bool F16, int HDP> struct PagedTile
@@ -57,6 +90,10 @@ template <bool F16, int HDP> struct PagedTile
     // probabilities as two parts, too: one part each cost 2^-12 on average in the result, as much as its own rounding does,
     // and the matrix cores have the time
     static constexpr int QN = F16 ? 2 : 1;
+    static constexpr int NP = kHeadsPerTile * HDP / 2 / 256; // query pairs that a thread stages
+    // Workgroups per CU. fp16, us with 1 / 2 / 3: 50 rows of up to 8192 over 5 key heads of 128 57 / 59 / 66, 200 rows of up
+    // to 500 over 9 39 / 36 / 43, 30 rows of up to 8192 over 5 of 256 82 / 94 / 103, 70 rows over 9 of 64 73 / 75 / 76
+    static constexpr int PER_CU = HDP == 256 ? 1 : 2;
 };
 
 __device__ __forceinline__ float exp2_of(float x)
@@ -64,320 +101,433 @@ __device__ __forceinline__ float exp2_of(float x)
     return __builtin_amdgcn_exp2f(x);
 }
 
+// the workgroup meets; what it wrote to LDS is seen. Loads from memory stay in flight, which __syncthreads would wait for.
+__device__ __forceinline__ void lds_barrier()
+{
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+}
+
 // dynamic LDS: lengths [B], queries [QN][16][QP], per-wave statistics [4][16][2], per-wave sums [4][tile_heads][hd]
-template <bool F16, int HDP> __global__ __launch_bounds__(256) void paged_attn_kernel(PagedAttnArgs a)
+// FULL: head_dim is HDP, else it is smaller
+template <bool F16, int HDP, bool FULL>
+__global__ __launch_bounds__(256, HDP == 256 ? 1 : HDP == 64 ? 4 : 2) void paged_attn_kernel(PagedAttnArgs a)
 {
     using Tile = PagedTile<F16, HDP>;
     using T = typename std::conditional<F16, _Float16, float>::type;
     constexpr int NT = Tile::NT, KW = Tile::KW, KT = Tile::KT, KS = Tile::KS, VD = Tile::VD, VW = Tile::VW,
-                  QP = Tile::QP, QN = Tile::QN;
+                  QP = Tile::QP, QN = Tile::QN, NP = Tile::NP;
+    constexpr uint32_t ES = sizeof(T);
     extern __shared__ uint32_t lds[];
     __shared__ uint64_t scan[4], first_unit;
-    __shared__ uint32_t first_row;
+    __shared__ uint32_t first_row, arrived;
+    __shared__ f32x4 joined[256];
+    // the rows whose parts lie in slots 0 and 1: how many parts they have, and the number of this one
+    struct Split
+    {
+        uint32_t b, hg, parts, number;
+    };
+    __shared__ Split split[2];
     const uint32_t t = threadIdx.x, lane = t % kWave, wave = __builtin_amdgcn_readfirstlane(t / kWave);
     const uint32_t g = lane / 16, c = lane % 16;
-    const uint32_t B = a.table.B, KV = a.cache.n[1] / 2, R = a.cache.n[2], hd = a.cache.n[3], H = a.q.n[2], G = H / KV;
+    const uint32_t B = a.table.B, hd = FULL ? HDP : a.hd, heads = a.KV * a.groups;
     uint32_t *lens = lds;
     T *qs = (T *)(lens + (B + 3) / 4 * 4);
     float *ml = (float *)(qs + QN * kHeadsPerTile * QP), *sums = ml + 4 * kHeadsPerTile * 2;
 
-    // units of every row, and this workgroup's run of them
-    const uint32_t per = (B + 255) / 256;
-    const uint64_t most = (uint64_t)a.table.P * R;
-    uint64_t mine = 0, total;
-    for (uint32_t b = t * per; b < t * per + per && b < B; ++b)
-    {
+    // rows of the queries that stay zero, and dims past the head
+    for (uint32_t i = t; i < QN * kHeadsPerTile * (QP / 4); i += 256)
+        if (i / (QP / 4) % kHeadsPerTile >= a.tile_heads || i % (QP / 4) * 4 >= hd)
+            for (uint32_t k = 0; k < 4; ++k)
+                qs[4 * i + k] = (T)0.f;
+    if (t < 2)
+        split[t].parts = 0;
+
+    // Units of every row, and this workgroup's run of them. A (sequence, head) counts `extra` units more, before its first:
+    // what starting and ending it costs. A sum holds units in its low 40 bits and rows that have any above.
+    const uint64_t most = (uint64_t)a.table.P * a.page_tiles * 16;
+    auto len_of = [&](uint32_t b) {
         const uint32_t len = a.table.p[(size_t)b * a.table.stride];
-        lens[b] = len > most ? (uint32_t)most : len;
-        mine += (uint64_t)((lens[b] + (uint64_t)KT - 1) / KT) * KV * a.groups;
-    }
-    for (uint32_t i = t; i < QN * kHeadsPerTile * QP; i += 256)
-        qs[i] = (T)0.f;
-    const uint64_t before = block_scan(mine, scan, total);
-    const uint64_t share = (total + gridDim.x - 1) / gridDim.x;
-    const uint64_t u0 = blockIdx.x * share, u1 = min(u0 + share, total);
-    if (u0 >= before && u0 < before + mine)
+        return len > most ? (uint32_t)most : len;
+    };
+    auto units_of = [&](uint32_t len) { return (uint32_t)((len + (uint64_t)KT - 1) / KT); };
+    auto count_of = [&](uint32_t len) { return units_of(len) | (uint64_t)(len > 0) << 40; };
+    uint32_t extra;
+    uint64_t share, u0, u1, base; // base: the number of the first row's first unit
+    uint32_t row0;                // the first row
+    auto weigh = [&](uint64_t sum) { return ((sum & ((1ull << 40) - 1)) + extra * (sum >> 40)) * heads; };
+    auto divide = [&](uint64_t total) {
+        extra = (total & ((1ull << 40) - 1)) * heads > 4 * gridDim.x ? kSegmentUnits : 0;
+        share = (weigh(total) + gridDim.x - 1) / gridDim.x;
+        u0 = blockIdx.x * share;
+        u1 = min(u0 + share, weigh(total));
+    };
+    if (B <= kWave)
     {
-        uint64_t at = before;
-        uint32_t b = t * per;
-        for (;; ++b)
-        {
-            const uint64_t n = (uint64_t)((lens[b] + (uint64_t)KT - 1) / KT) * KV * a.groups;
-            if (u0 < at + n)
-                break;
-            at += n;
-        }
-        first_unit = at;
-        first_row = b;
+        // every wave for itself
+        const uint32_t len = lane < B ? len_of(lane) : 0;
+        if (lane < B)
+            lens[lane] = len;
+        const uint64_t mine = count_of(len), upto = wave_scan(mine);
+        divide(read_lane(upto, kWave - 1));
+        const uint64_t found = __ballot(u0 < weigh(upto) && u0 >= weigh(upto - mine));
+        row0 = found ? __ffsll((unsigned long long)found) - 1 : 0;
+        base = weigh(read_lane(upto - mine, row0));
     }
-    __syncthreads();
+    else
+    {
+        const uint32_t per = (B + 255) / 256;
+        uint64_t mine = 0, total;
+        for (uint32_t b = t * per; b < t * per + per && b < B; ++b)
+        {
+            lens[b] = len_of(b);
+            mine += count_of(lens[b]);
+        }
+        uint64_t at = block_scan(mine, scan, total);
+        divide(total);
+        if (u0 >= weigh(at) && u0 < weigh(at + mine))
+        {
+            uint32_t b = t * per;
+            for (; u0 >= weigh(at + count_of(lens[b])); ++b)
+                at += count_of(lens[b]);
+            first_unit = weigh(at);
+            first_row = b;
+        }
+        __syncthreads();
+        row0 = first_row;
+        base = first_unit;
+    }
     // sequences without a token
     for (uint32_t b = blockIdx.x; b < B; b += gridDim.x)
         if (lens[b] == 0)
-            for (uint32_t e = t; e < H * hd; e += 256)
-                ((T *)a.out.p)[(size_t)b * a.out.s[1] + (size_t)(e / hd) * a.out.s[2] + (size_t)(e % hd) * a.out.s[3]] =
-                    (T)0.f;
-    if (t == 0)
-        a.joins[blockIdx.x * 4] = 0;
+            for (uint32_t e = t; e < a.KV * a.G * hd; e += 256)
+                ((T *)a.out)[(size_t)b * a.os[0] + (size_t)(e / hd) * a.os[1] + (size_t)(e % hd) * a.os[2]] = (T)0.f;
     if (u0 >= u1)
         return;
 
-    uint64_t base = first_unit;
-    uint32_t b = first_row;
-    for (uint64_t u = u0; u < u1;)
+    // A unit's place: sequence b of `len` positions and n units per head, tile hg of its query heads, unit s of number v. The
+    // same for the whole workgroup, so it is kept in scalar registers.
+    struct Place
     {
-        const uint32_t len = lens[b], n_units = (uint32_t)((len + (uint64_t)KT - 1) / KT);
-        const uint64_t row_units = (uint64_t)n_units * KV * a.groups;
-        if (u >= base + row_units)
+        uint32_t b, len, n, hg, s;
+        uint32_t v; // behind u0
+    };
+    auto row_at = [&](Place &p, uint32_t b) {
+        do
+            p.len = __builtin_amdgcn_readfirstlane(lens[b]);
+        while (p.len == 0 && ++b < B);
+        p.b = b;
+        p.n = units_of(p.len);
+    };
+    auto next_of = [&](Place p) {
+        ++p.v;
+        if (++p.s == p.n)
         {
-            base += row_units;
-            ++b;
-            continue;
-        }
-        const uint32_t hg = (uint32_t)((u - base) / n_units), s0 = (uint32_t)((u - base) % n_units);
-        const uint32_t s1 = (uint32_t)min((uint64_t)n_units, s0 + (u1 - u));
-        const uint32_t h = hg / a.groups, head0 = h * G + hg % a.groups * kHeadsPerTile;
-        const uint32_t Gn = min((uint32_t)kHeadsPerTile, (h + 1) * G - head0);
-
-        // queries into LDS, rotated to the last position
-        for (uint32_t e = t; e < Gn * (hd / 2); e += 256)
-        {
-            const uint32_t i = e / (hd / 2), w = e % (hd / 2);
-            const uint32_t d0 = a.rope.style == 1 ? 2 * w : w, d1 = a.rope.style == 1 ? 2 * w + 1 : w + hd / 2;
-            const T *q = (const T *)a.q.p + (size_t)b * a.q.s[1] + (size_t)(head0 + i) * a.q.s[2];
-            const float x = (float)q[(size_t)d0 * a.q.s[3]], y = (float)q[(size_t)d1 * a.q.s[3]];
-            float u = x, v = y;
-            if (a.rope.style)
+            p.s = 0;
+            p.v += extra;
+            if (++p.hg == heads)
             {
-                const float2 r = turn_at(len - 1, a.rope.turns[w]);
-                u = r.x * x - r.y * y;
-                v = r.y * x + r.x * y;
-                if constexpr (F16)
-                {
-                    u *= 0.5f;
-                    v *= 0.5f;
-                    qs[(kHeadsPerTile + i) * QP + d0] = (T)(u - (float)(T)u);
-                    qs[(kHeadsPerTile + i) * QP + d1] = (T)(v - (float)(T)v);
-                }
+                p.hg = 0;
+                row_at(p, min(p.b + 1, B - 1));
             }
-            qs[i * QP + d0] = (T)u;
-            qs[i * QP + d1] = (T)v;
         }
-        __syncthreads();
-        u32x4 qf[QN][KS];
+        return p;
+    };
+    Place cur;
+    row_at(cur, __builtin_amdgcn_readfirstlane(row0));
+    {
+        const uint64_t rel = u0 - base, n = cur.n + extra;
+        const uint32_t at = (uint32_t)(rel % n);
+        cur.hg = __builtin_amdgcn_readfirstlane((uint32_t)(rel / n));
+        cur.s = __builtin_amdgcn_readfirstlane(at < extra ? 0 : at - extra);
+        cur.v = __builtin_amdgcn_readfirstlane(at < extra ? extra - at : 0);
+    }
+    const uint32_t end = __builtin_amdgcn_readfirstlane((uint32_t)(u1 - u0));
+    if (cur.v >= end)
+        return;
+
+    auto head_of = [&](const Place &p) { return p.hg / a.groups; };
+    auto head0_of = [&](const Place &p) { return head_of(p) * a.G + p.hg % a.groups * kHeadsPerTile; };
+    auto heads_of = [&](const Place &p) { return min((uint32_t)kHeadsPerTile, (head_of(p) + 1) * a.G - head0_of(p)); };
+
+    // Queries and their pairs' frequencies: thread t has pairs t + 256 j of tile_heads heads (the other rows in LDS stay
+    // zero). They are asked for before the keys of their first unit, and staged when the unit before is done with.
+    T qx[NP], qy[NP];
+    double turns[NP];
+    auto pair_dims = [&](uint32_t w, uint32_t &d0, uint32_t &d1) {
+        d0 = a.rope.style == 1 ? 2 * w : w;
+        d1 = a.rope.style == 1 ? 2 * w + 1 : w + hd / 2;
+    };
+    auto load_q = [&](const Place &p) {
+        const uint32_t head0 = head0_of(p), Gn = heads_of(p);
 #pragma unroll
-        for (int n = 0; n < QN; ++n)
+        for (int j = 0; j < NP; ++j)
+            if (256 * j < a.tile_heads * (hd / 2))
+            {
+                const uint32_t e = t + 256 * j, i = e / (hd / 2), w = e % (hd / 2);
+                uint32_t d0, d1;
+                pair_dims(w, d0, d1);
+                const T *q = (const T *)a.q + (size_t)p.b * a.qs[0] + (size_t)(head0 + (i < Gn ? i : 0)) * a.qs[1];
+                qx[j] = q[(size_t)d0 * a.qs[2]];
+                qy[j] = q[(size_t)d1 * a.qs[2]];
+                turns[j] = a.rope.turns[w];
+            }
+    };
+    auto stage_q = [&](const Place &p) {
+        const uint32_t Gn = heads_of(p);
+#pragma unroll
+        for (int j = 0; j < NP; ++j)
+            if (256 * j < a.tile_heads * (hd / 2))
+            {
+                const uint32_t e = t + 256 * j, i = e / (hd / 2), w = e % (hd / 2);
+                uint32_t d0, d1;
+                pair_dims(w, d0, d1);
+                float u = i < Gn ? (float)qx[j] : 0.f, v = i < Gn ? (float)qy[j] : 0.f;
+                if (i >= a.tile_heads)
+                    continue;
+                if (a.rope.style)
+                {
+                    const float2 r = turn_at(p.len - 1, turns[j]);
+                    const float x = u, y = v;
+                    u = r.x * x - r.y * y;
+                    v = r.y * x + r.x * y;
+                    if constexpr (F16)
+                    {
+                        u *= 0.5f;
+                        v *= 0.5f;
+                        qs[(kHeadsPerTile + i) * QP + d0] = (T)(u - (float)(T)u);
+                        qs[(kHeadsPerTile + i) * QP + d1] = (T)(v - (float)(T)v);
+                    }
+                }
+                qs[i * QP + d0] = (T)u;
+                qs[i * QP + d1] = (T)v;
+            }
+    };
+
+    // pages of the wave's tiles in a unit
+    uint32_t pid[NT];
+    auto tile_of = [&](const Place &p, int i) { return (p.s * KT + wave * KW) / 16 + i; };
+    auto page_of = [&](uint32_t tile) { return (uint32_t)((uint64_t)tile * a.div_magic >> a.div_shift); };
+    auto fetch = [&](const Place &p) {
+        const uint32_t *row = a.table.p + (size_t)p.b * a.table.stride + 1;
+#pragma unroll
+        for (int i = 0; i < NT; ++i)
+            pid[i] = scalar_word(row + page_of(min(tile_of(p, i), (p.len - 1) / 16)));
+    };
+    // A tile's rows start at an address of the wave, to which every lane adds an offset of its own that never changes.
+    const char *rows[NT];
+    uint32_t live[NT]; // the tiles' keys
+    auto place = [&](const Place &p) {
+#pragma unroll
+        for (int i = 0; i < NT; ++i)
+        {
+            const uint32_t tile = tile_of(p, i);
+            // past the end, or an absent page: read page 0, use nothing of it
+            const bool there = tile <= (p.len - 1) / 16 && pid[i] < a.pages;
+            live[i] = there ? min(16u, p.len - tile * 16) : 0u;
+            const uint32_t in_page = tile - page_of(tile) * a.page_tiles;
+            const size_t at = (size_t)pid[i] * a.page_bytes + (head_of(p) * a.head_bytes + in_page * (16 * hd * ES));
+            rows[i] = (const char *)a.cache + (there ? at : 0);
+        }
+    };
+    u32x4 kr[NT][KS];
+    uint32_t vr[NT * 4][VW];
+    auto load_k = [&]() {
+#pragma unroll
+        for (int i = 0; i < NT; ++i)
 #pragma unroll
             for (int s = 0; s < KS; ++s)
-                qf[n][s] = c < Gn ? *(const u32x4 *)(qs + (n * kHeadsPerTile + c) * QP +
-                                                     (F16 ? 8 * (g + 4 * s) : 16 * s + 4 * g))
-                                  : (u32x4){0, 0, 0, 0};
+            {
+                const uint32_t d = 16 * g + 64 * s; // bytes
+                kr[i][s] = *(const u32x4 *)(rows[i] + (c * hd * ES + (FULL || d < hd * ES ? d : 0)));
+            }
+    };
+    auto load_v = [&]() {
+#pragma unroll
+        for (int i = 0; i < NT; ++i)
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+            {
+                uint32_t *to = vr[4 * i + r];
+                const char *p = rows[i] + (size_t)a.KV * a.head_bytes + r * hd * ES;
+                if constexpr (VW == 2)
+                {
+                    const uint32_t d = 8 * c;
+                    const uint2 v = *(const uint2 *)(p + (4 * g * hd * ES + (FULL || d < hd * ES ? d : 0)));
+                    to[0] = v.x;
+                    to[1] = v.y;
+                }
+                else
+                {
+#pragma unroll
+                    for (int w = 0; w < VW / 4; ++w)
+                    {
+                        const uint32_t d = VD * ES * c + 16 * w;
+                        const u32x4 v = *(const u32x4 *)(p + (4 * g * hd * ES + (FULL || d < hd * ES ? d : 0)));
+#pragma unroll
+                        for (int k = 0; k < 4; ++k)
+                            to[4 * w + k] = v[k];
+                    }
+                }
+            }
+    };
 
-        float m = kNegInf, l = 0.f;
-        f32x4 o[VD];
+    float m, l;
+    f32x4 o[VD];
+    auto clear = [&]() {
+        m = kNegInf;
+        l = 0.f;
 #pragma unroll
         for (int d = 0; d < VD; ++d)
             o[d] = (f32x4){0.f, 0.f, 0.f, 0.f};
-        const uint32_t *row = a.table.p + (size_t)b * a.table.stride + 1;
-        uint32_t pid[NT]; // pages of the step after the one that is being loaded
-        auto fetch = [&](uint32_t s) {
+    };
+    uint32_t q_at = c * QP + (F16 ? 8 : 4) * g;
+
+    // One unit; `more`: with the loads of the unit `next` (and the pages of the one `after` it). The last unit is code of its own, because
+    // where paths with and without newer loads meet, the compiler waits for all of them.
+    auto step = [&](auto more, const Place &next, const Place &after) {
+        constexpr bool MORE = decltype(more)::value;
+        // read again at every step (the compiler is kept from moving that out of the loop): in registers the queries would
+        // cost half of the resident waves
+        asm volatile("" : "+v"(q_at));
+        auto query = [&](int n, int s) { return *(const u32x4 *)(qs + q_at + n * kHeadsPerTile * QP + (F16 ? 32 : 16) * s); };
+        f32x4 x[NT];
 #pragma unroll
-            for (int i = 0; i < NT; ++i)
-            {
-                const uint32_t key = s * KT + wave * KW + 16 * i;
-                pid[i] = s < s1 && key < len ? row[key / R] : kNoPage;
-            }
-        };
-        const T *rows[NT]; // the tiles' first key rows
-        uint32_t live[NT]; // their keys
-        auto place = [&](uint32_t s) {
+        for (int i = 0; i < NT; ++i)
+            x[i] = (f32x4){0.f, 0.f, 0.f, 0.f};
+        if constexpr (!FULL)
 #pragma unroll
-            for (int i = 0; i < NT; ++i)
-            {
-                const uint32_t key = s * KT + wave * KW + 16 * i;
-                const bool there = pid[i] < a.cache.n[0]; // absent pages: read page 0, use nothing of it
-                live[i] = there ? min(16u, len - key) : 0u;
-                rows[i] = (const T *)a.cache.p +
-                          (there ? (size_t)pid[i] * a.cache.s[0] + (size_t)h * a.cache.s[1] + (size_t)(key % R) * hd : 0);
-            }
-        };
-        u32x4 kr[NT][KS];
-        uint32_t vr[NT * 4][VW];
-        auto load_k = [&]() {
+            for (int k = 0; k < KS; ++k)
+                if (16 * g + 64 * k >= hd * ES) // past the row: not a number for sure
 #pragma unroll
-            for (int i = 0; i < NT; ++i)
-#pragma unroll
-                for (int s = 0; s < KS; ++s)
-                {
-                    const uint32_t d = F16 ? 8 * (g + 4 * s) : 16 * s + 4 * g;
-                    kr[i][s] = *(const u32x4 *)(rows[i] + c * hd + (d < hd ? d : 0));
-                }
-        };
-        const T *vrows[NT];
-        auto load_v = [&]() {
-#pragma unroll
-            for (int i = 0; i < NT; ++i)
-#pragma unroll
-                for (int r = 0; r < 4; ++r)
-                {
-                    const T *p = vrows[i] + (4 * g + r) * hd;
-                    uint32_t *to = vr[4 * i + r];
-                    if constexpr (VW == 2)
-                    {
-                        const uint2 v = *(const uint2 *)(p + (4 * c < hd ? 4 * c : 0));
-                        to[0] = v.x;
-                        to[1] = v.y;
-                    }
-                    else
-                    {
-#pragma unroll
-                        for (int w = 0; w < VW / 4; ++w)
-                        {
-                            const uint32_t d = VD * c + (F16 ? 8 : 4) * w;
-                            const u32x4 v = *(const u32x4 *)(p + (d < hd ? d : 0));
-#pragma unroll
-                            for (int k = 0; k < 4; ++k)
-                                to[4 * w + k] = v[k];
-                        }
-                    }
-                }
-        };
-        auto point_v = [&]() {
-#pragma unroll
-            for (int i = 0; i < NT; ++i)
-                vrows[i] = rows[i] + (size_t)KV * a.cache.s[1];
-        };
-        fetch(s0);
-        place(s0);
-        load_k();
-        point_v();
-        load_v();
-        fetch(s0 + 1);
-        for (uint32_t s = s0; s < s1; ++s)
+                    for (int i = 0; i < NT; ++i)
+                        kr[i][k] = (u32x4){0, 0, 0, 0};
+        if constexpr (F16)
         {
-            f32x4 x[NT];
-#pragma unroll
-            for (int i = 0; i < NT; ++i)
-            {
-                x[i] = (f32x4){0.f, 0.f, 0.f, 0.f};
+            auto score = [&](int n) {
 #pragma unroll
                 for (int k = 0; k < KS; ++k)
                 {
-                    u32x4 kv = kr[i][k];
-                    if (hd != HDP && (F16 ? 8 * (g + 4 * k) : 16 * k + 4 * g) >= hd)
-                        kv = (u32x4){0, 0, 0, 0};
-                    if constexpr (F16)
-                    {
-                        x[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
-                            __builtin_bit_cast(half8, kv), __builtin_bit_cast(half8, qf[0][k]), x[i], 0, 0, 0);
-                        if (a.rope.style)
-                            x[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
-                                __builtin_bit_cast(half8, kv), __builtin_bit_cast(half8, qf[1][k]), x[i], 0, 0, 0);
-                    }
-                    else
-                    {
+                    const half8 q = __builtin_bit_cast(half8, query(n, k));
 #pragma unroll
-                        for (int e = 0; e < 4; ++e)
-                            x[i] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(kv[e]),
-                                                                        __uint_as_float(qf[0][k][e]), x[i], 0, 0, 0);
-                    }
+                    for (int i = 0; i < NT; ++i)
+                        x[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8, kr[i][k]), q, x[i], 0, 0, 0);
                 }
-            }
-            uint32_t n[NT];
+            };
+            score(0);
+            if (a.rope.style)
+                score(1);
+        }
+        else
+        {
 #pragma unroll
-            for (int i = 0; i < NT; ++i)
-                n[i] = live[i];
-            const bool more = s + 1 < s1;
-            if (more)
+            for (int k = 0; k < KS; ++k)
             {
-                place(s + 1);
-                load_k();
-                fetch(s + 2);
-            }
-            bool whole = true;
+                const u32x4 q = query(0, k);
 #pragma unroll
-            for (int i = 0; i < NT; ++i)
-                whole = whole && n[i] == 16;
-            float top = kNegInf;
-#pragma unroll
-            for (int i = 0; i < NT; ++i)
-#pragma unroll
-                for (int r = 0; r < 4; ++r)
-                {
-                    x[i][r] *= a.scale_log2;
-                    if (!whole && 4 * g + r >= n[i])
-                        x[i][r] = kNegInf;
-                    top = fmaxf(top, x[i][r]);
-                }
-            // m rises when a score passes it by 7: probabilities then stay below 2^15 at the 2^8 that fp16 ones are scaled
-            // by, and those down to 2^-32 of the largest still count
-            if (__any(top > m + 7.f))
-            {
-                top = fmaxf(top, __shfl_xor(top, 16, kWave));
-                top = fmaxf(top, __shfl_xor(top, 32, kWave));
-                const float next = fmaxf(m, top), f = m == kNegInf ? 0.f : exp2_of(m - next);
-                m = next;
-                l *= f;
-#pragma unroll
-                for (int d = 0; d < VD; ++d)
-                    o[d] *= f;
-            }
-            const float ref = m == kNegInf ? 0.f : m - (F16 ? 8.f : 0.f);
-#pragma unroll
-            for (int i = 0; i < NT; ++i)
-#pragma unroll
-                for (int r = 0; r < 4; ++r)
-                {
-                    x[i][r] = exp2_of(x[i][r] - ref);
-                    l += x[i][r];
-                }
-            if (!whole) // what lies past the end is not a number for sure
-            {
-#pragma unroll
-                for (int i = 0; i < NT; ++i)
-#pragma unroll
-                    for (int r = 0; r < 4; ++r)
-#pragma unroll
-                        for (int w = 0; w < VW; ++w)
-                            vr[4 * i + r][w] = 4 * g + r < n[i] ? vr[4 * i + r][w] : 0u;
-            }
-            if constexpr (F16)
-            {
-                half8 p, q; // p's rest
-#pragma unroll
-                for (int j = 0; j < 8; ++j)
-                {
-                    p[j] = (_Float16)x[j / 4][j % 4];
-                    q[j] = (_Float16)(x[j / 4][j % 4] - (float)p[j]);
-                }
-#pragma unroll
-                for (int d = 0; d < VD; ++d)
-                {
-                    u32x4 v; // 8 keys of dim VD * c + d
-#pragma unroll
-                    for (int j = 0; j < 4; ++j)
-                        v[j] = __builtin_amdgcn_perm(vr[2 * j + 1][d / 2], vr[2 * j][d / 2],
-                                                     d % 2 ? 0x07060302u : 0x05040100u);
-                    o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8, v), p, o[d], 0, 0, 0);
-                    o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8, v), q, o[d], 0, 0, 0);
-                }
-            }
-            else
-            {
-#pragma unroll
-                for (int r = 0; r < 4; ++r)
-#pragma unroll
-                    for (int d = 0; d < VD; ++d)
-                        o[d] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(vr[r][d]), x[0][r], o[d], 0, 0, 0);
-            }
-            if (more)
-            {
-                point_v();
-                load_v();
+                for (int e = 0; e < 4; ++e)
+                    x[0] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(kr[0][k][e]), __uint_as_float(q[e]), x[0], 0,
+                                                                0, 0);
             }
         }
+        uint32_t n[NT];
+        bool whole = true;
+#pragma unroll
+        for (int i = 0; i < NT; ++i)
+        {
+            n[i] = live[i];
+            whole = whole && n[i] == 16;
+        }
+        if constexpr (MORE)
+        {
+            place(next);
+            if (next.s == 0)
+                load_q(next);
+            load_k();
+            fetch(after);
+        }
+        float top = kNegInf;
+#pragma unroll
+        for (int i = 0; i < NT; ++i)
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+            {
+                x[i][r] *= a.scale_log2;
+                if (!whole && 4 * g + r >= n[i])
+                    x[i][r] = kNegInf;
+                top = fmaxf(top, x[i][r]);
+            }
+        // m rises when a score passes it by 7: probabilities then stay below 2^15 at the 2^8 that fp16 ones are scaled by, and
+        // those down to 2^-32 of the largest still count
+        if (__any(top > m + 7.f))
+        {
+            top = fmaxf(top, __shfl_xor(top, 16, kWave));
+            top = fmaxf(top, __shfl_xor(top, 32, kWave));
+            const float high = fmaxf(m, top), f = m == kNegInf ? 0.f : exp2_of(m - high);
+            m = high;
+            l *= f;
+#pragma unroll
+            for (int d = 0; d < VD; ++d)
+                o[d] *= f;
+        }
+        const float ref = m == kNegInf ? 0.f : m - (F16 ? 8.f : 0.f);
+#pragma unroll
+        for (int i = 0; i < NT; ++i)
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+            {
+                x[i][r] = exp2_of(x[i][r] - ref);
+                l += x[i][r];
+            }
+        if (!whole) // what lies past the end is not a number for sure
+        {
+#pragma unroll
+            for (int i = 0; i < NT; ++i)
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+#pragma unroll
+                    for (int w = 0; w < VW; ++w)
+                        vr[4 * i + r][w] = 4 * g + r < n[i] ? vr[4 * i + r][w] : 0u;
+        }
+        if constexpr (F16)
+        {
+            half8 p, q; // p's rest
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+            {
+                p[j] = (_Float16)x[j / 4][j % 4];
+                q[j] = (_Float16)(x[j / 4][j % 4] - (float)p[j]);
+            }
+#pragma unroll
+            for (int d = 0; d < VD; ++d)
+            {
+                u32x4 v; // 8 keys of dim VD * c + d
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    v[j] = __builtin_amdgcn_perm(vr[2 * j + 1][d / 2], vr[2 * j][d / 2], d % 2 ? 0x07060302u : 0x05040100u);
+                o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8, v), p, o[d], 0, 0, 0);
+                o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8, v), q, o[d], 0, 0, 0);
+            }
+        }
+        else
+        {
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+#pragma unroll
+                for (int d = 0; d < VD; ++d)
+                    o[d] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(vr[r][d]), x[0][r], o[d], 0, 0, 0);
+        }
+        if constexpr (MORE)
+            load_v();
+    };
 
-        // the four waves' sums
+    auto store_out = [&](uint32_t b, uint32_t head, uint32_t d, float o0, float o1, float lsum) {
+        T *to = (T *)a.out + (size_t)b * a.os[0] + (size_t)head * a.os[1] + (size_t)d * a.os[2];
+        to[0] = (T)(lsum == 0.f ? 0.f : o0 / lsum); // a row of no weight is zero
+        to[a.os[2]] = (T)(lsum == 0.f ? 0.f : o1 / lsum);
+    };
+    // What the workgroup has of (sequence, heads) p.b, p.hg: its units from `from` to p.s
+    auto finish = [&](const Place &p, uint32_t from) {
+        const uint32_t Gn = heads_of(p), head0 = head0_of(p);
         l += __shfl_xor(l, 16, kWave);
         l += __shfl_xor(l, 32, kWave);
         if (c < Gn)
@@ -392,16 +542,17 @@ template <bool F16, int HDP> __global__ __launch_bounds__(256) void paged_attn_k
             for (int i = 0; i < 4; ++i)
 #pragma unroll
                 for (int d = 0; d < VD; ++d)
-                    if (VD * (4 * g + i) + d < hd)
+                    if (FULL || VD * (4 * g + i) + d < hd)
                         to[VD * (4 * g + i) + d] = o[d][i];
         }
-        __syncthreads();
-        const bool all = s0 == 0 && s1 == n_units;
-        float *part = a.parts + (2 * (size_t)blockIdx.x + (u == u0 ? 0 : 1)) * part_floats(a.tile_heads, hd);
-        for (uint32_t e = t; e < Gn * hd; e += 256)
+        lds_barrier();
+        const bool all = from == 0 && p.s + 1 == p.n;
+        // a row that began in another workgroup leaves its part in slot 0, one that goes on in the next in slot 1
+        float *part = a.parts + (2 * (size_t)blockIdx.x + (from == 0 ? 1 : 0)) * part_floats(a.tile_heads, hd);
+        for (uint32_t e = 2 * t; e < Gn * hd; e += 512)
         {
             const uint32_t i = e / hd, d = e % hd;
-            float mw[4], top = kNegInf, lsum = 0.f, osum = 0.f;
+            float mw[4], top = kNegInf, lsum = 0.f, o0 = 0.f, o1 = 0.f;
 #pragma unroll
             for (int w = 0; w < 4; ++w)
             {
@@ -412,129 +563,238 @@ template <bool F16, int HDP> __global__ __launch_bounds__(256) void paged_attn_k
             for (int w = 0; w < 4; ++w)
             {
                 const float f = mw[w] == kNegInf ? 0.f : exp2_of(mw[w] - top);
+                const float *sum = sums + (size_t)(w * a.tile_heads + i) * hd + d;
                 lsum += f * ml[(w * kHeadsPerTile + i) * 2 + 1];
-                osum += f * sums[(size_t)(w * a.tile_heads + i) * hd + d];
+                o0 += f * sum[0];
+                o1 += f * sum[1];
             }
             if (all)
-                ((T *)a.out.p)[(size_t)b * a.out.s[1] + (size_t)(head0 + i) * a.out.s[2] + (size_t)d * a.out.s[3]] =
-                    (T)(lsum == 0.f ? 0.f : osum / lsum);
+                store_out(p.b, head0 + i, d, o0, o1, lsum);
             else
             {
-                part[2 * a.tile_heads + i * hd + d] = osum;
+                put2(part + e, o0, o1);
                 if (d == 0)
-                {
-                    part[i] = top;
-                    part[a.tile_heads + i] = lsum;
-                }
+                    put2(part + a.tile_heads * hd + 2 * i, top, lsum);
             }
         }
-        // the workgroup with the first units of a row that goes on has it joined
-        if (!all && s0 == 0 && t == 0)
+    };
+
+    load_q(cur);
+    fetch(cur);
+    place(cur);
+    load_k();
+    load_v();
+    Place next = next_of(cur);
+    if (next.v < end)
+        fetch(next);
+    stage_q(cur);
+    clear();
+    lds_barrier();
+    uint32_t from = cur.s;
+    auto note = [&](const Place &p, uint32_t from) {
+        const uint32_t before = (uint32_t)((from + share - 1) / share), behind = (uint32_t)((p.n - p.s - 1 + share - 1) / share);
+        if (t == 0)
+            split[from == 0] = {p.b, p.hg, before + 1 + behind, before};
+    };
+    while (next.v < end)
+    {
+        const Place after = next_of(next); // with v >= end, another workgroup's or none
+        step(std::true_type(), next, after.v < end ? after : next);
+        if (next.s == 0)
         {
-            const uint64_t last = base + (uint64_t)hg * n_units + n_units - 1;
-            a.joins[blockIdx.x * 4] = (uint32_t)(last / share) - blockIdx.x + 1;
-            a.joins[blockIdx.x * 4 + 1] = b;
-            a.joins[blockIdx.x * 4 + 2] = hg;
-            a.joins[blockIdx.x * 4 + 3] = u == u0 ? 0 : 1;
+            finish(cur, from);
+            if (from != 0)
+                note(cur, from);
+            stage_q(next);
+            clear();
+            from = 0;
+            lds_barrier();
         }
-        u += s1 - s0;
+        cur = next;
+        next = after;
     }
-}
+    step(std::false_type(), cur, cur);
+    finish(cur, from);
+    if (from != 0 || cur.s + 1 < cur.n)
+        note(cur, from);
 
-// Joins the partial results of the row that begins in workgroup x of the kernel above and goes on in those after it (its
-// first part in slot joins[3], the others in slot 0); workgroup (x, i) has query head i of the tile.
-template <bool F16> __global__ __launch_bounds__(256) void paged_join_kernel(PagedAttnArgs a)
-{
-    using T = typename std::conditional<F16, _Float16, float>::type;
-    __shared__ float sums[4][kPagedMaxHd];
-    const uint32_t *join = a.joins + blockIdx.x * 4;
-    const uint32_t n = join[0], i = blockIdx.y;
-    if (n == 0)
-        return;
-    const uint32_t b = join[1], hg = join[2], slot = join[3];
-    const uint32_t KV = a.cache.n[1] / 2, hd = a.cache.n[3], G = a.q.n[2] / KV, h = hg / a.groups;
-    const uint32_t head = h * G + hg % a.groups * kHeadsPerTile + i;
-    if (head >= (h + 1) * G)
-        return;
-    const uint32_t t = threadIdx.x, lane = t % kWave, wave = t / kWave;
-    const size_t floats = part_floats(a.tile_heads, hd);
-    auto part = [&](uint32_t k) { return a.parts + (2 * (size_t)(blockIdx.x + k) + (k == 0 ? slot : 0)) * floats; };
-    float top = kNegInf;
-    for (uint32_t k = lane; k < n; k += kWave)
-        top = fmaxf(top, part(k)[i]);
-    top = wave_max(top);
-    float lsum = 0.f;
-    for (uint32_t k = lane; k < n; k += kWave)
-    {
-        const float mk = part(k)[i];
-        lsum += mk == kNegInf ? 0.f : exp2_of(mk - top) * part(k)[a.tile_heads + i];
-    }
-    lsum = wave_sum(lsum);
-    float o[kPagedMaxHd / kWave] = {};
-#pragma unroll 4
-    for (uint32_t k = wave; k < n; k += 4)
-    {
-        const float *p = part(k);
-        const float f = p[i] == kNegInf ? 0.f : exp2_of(p[i] - top);
-#pragma unroll
-        for (int j = 0; j < kPagedMaxHd / kWave; ++j)
-            if (lane + j * kWave < hd)
-                o[j] += f * p[2 * a.tile_heads + i * hd + lane + j * kWave];
-    }
-#pragma unroll
-    for (int j = 0; j < kPagedMaxHd / kWave; ++j)
-        if (lane + j * kWave < hd)
-            sums[wave][lane + j * kWave] = o[j];
+    // Joins. Parts that lie next to each other form groups of `fan`; the last workgroup of a group to arrive (no workgroup
+    // waits for another) joins its parts in their order, into the first one's place, and arrives for the group at the next
+    // level. Which parts are joined with which depends on the lengths alone, so results do not hang on the arrivals' order.
     __syncthreads();
-    if (t < hd)
+#pragma unroll 1
+    for (int which = 0; which < 2; ++which)
     {
-        const float osum = (sums[0][t] + sums[1][t]) + (sums[2][t] + sums[3][t]);
-        ((T *)a.out.p)[(size_t)b * a.out.s[1] + (size_t)head * a.out.s[2] + (size_t)t * a.out.s[3]] =
-            (T)(lsum == 0.f ? 0.f : osum / lsum);
+        uint32_t n = __builtin_amdgcn_readfirstlane(split[which].parts);
+        if (n == 0)
+            continue;
+        const uint32_t hg = __builtin_amdgcn_readfirstlane(split[which].hg), head0 = hg / a.groups * a.G + hg % a.groups * kHeadsPerTile;
+        const uint32_t Gn = min((uint32_t)kHeadsPerTile, (hg / a.groups + 1) * a.G - head0);
+        uint32_t k = __builtin_amdgcn_readfirstlane(split[which].number), stride = 1;
+        const uint32_t first = blockIdx.x - k, pairs = Gn * hd / 2;
+        const uint32_t ways = join_ways(pairs), fan = kJoinFan * ways;
+        const size_t floats = part_floats(a.tile_heads, hd), half = 2 * gridDim.x * floats;
+        // the place of part k: the first part's row starts in its workgroup, the others' does not
+        auto slot = [&](uint32_t k) { return 2 * (size_t)(first + k) + (k == 0 ? 1 : 0); };
+        for (uint32_t level = 0;; ++level)
+        {
+            const uint32_t group = k / fan, size = min(fan, n - group * fan), lead = group * fan * stride;
+            __builtin_amdgcn_s_waitcnt(0); // what this thread wrote of the part is there
+            __syncthreads();
+            if (t == 0)
+            {
+                uint32_t *counter = a.arrivals + 2 * (size_t)level * gridDim.x + slot(lead);
+                arrived = __hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                if (arrived == size - 1)
+                    __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); // for the next launch
+            }
+            __syncthreads();
+            if (arrived != size - 1)
+                break;
+            // levels write one half of the workspace and read the other, so nothing is overwritten that is still read
+            const float *in = a.parts + (level % 2) * half;
+            float *to = a.parts + (1 - level % 2) * half + slot(lead) * floats;
+            // (m, l, o, o) of pair e from parts way, way + ways, ... of the group
+            auto gather = [&](uint32_t e, uint32_t way) {
+                float2 o[kJoinFan], ml[kJoinFan];
+#pragma unroll
+                for (uint32_t c = 0; c < kJoinFan; ++c)
+                {
+                    const float *part = in + slot(lead + min(way + c * ways, size - 1) * stride) * floats;
+                    o[c] = get2(part + 2 * e);
+                    ml[c] = get2(part + a.tile_heads * hd + 2 * (2 * e / hd));
+                }
+                float m = kNegInf;
+#pragma unroll
+                for (uint32_t c = 0; c < kJoinFan; ++c)
+                {
+                    if (way + c * ways >= size)
+                        ml[c].x = kNegInf;
+                    m = fmaxf(m, ml[c].x);
+                }
+                f32x4 r = {m, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (uint32_t c = 0; c < kJoinFan; ++c)
+                    if (ml[c].x != kNegInf)
+                    {
+                        const float f = exp2_of(ml[c].x - m);
+                        r[1] += f * ml[c].y;
+                        r[2] += f * o[c].x;
+                        r[3] += f * o[c].y;
+                    }
+                return r;
+            };
+            auto emit = [&](uint32_t e, f32x4 r) {
+                const uint32_t i = 2 * e / hd, d = 2 * e % hd;
+                if (n <= fan)
+                    store_out(split[which].b, head0 + i, d, r[2], r[3], r[1]);
+                else
+                {
+                    put2(to + 2 * e, r[2], r[3]);
+                    if (d == 0)
+                        put2(to + a.tile_heads * hd + 2 * i, r[0], r[1]);
+                }
+            };
+            if (ways == 1)
+                for (uint32_t e = t; e < pairs; e += 256)
+                    emit(e, gather(e, 0));
+            else
+            {
+                if (t < ways * pairs)
+                    joined[t] = gather(t % pairs, t / pairs);
+                __syncthreads();
+                if (t < pairs)
+                {
+                    float m = kNegInf;
+                    for (uint32_t w = 0; w < ways; ++w)
+                        m = fmaxf(m, joined[w * pairs + t][0]);
+                    f32x4 r = {m, 0.f, 0.f, 0.f};
+                    for (uint32_t w = 0; w < ways; ++w)
+                    {
+                        const f32x4 x = joined[w * pairs + t];
+                        if (x[0] != kNegInf)
+                        {
+                            const float f = exp2_of(x[0] - m);
+                            r[1] += f * x[1];
+                            r[2] += f * x[2];
+                            r[3] += f * x[3];
+                        }
+                    }
+                    emit(t, r);
+                }
+            }
+            if (n <= fan)
+                break;
+            k = group;
+            n = (n - 1) / fan + 1;
+            stride *= fan;
+        }
     }
 }
 
-template <bool F16, int HDP>
-static hipError_t launch_as(hipStream_t st, PagedAttnArgs &a, float *work, size_t work_elems, int cu_count)
+template <bool F16, int HDP, bool FULL>
+static hipError_t launch_as(hipStream_t st, PagedAttnArgs &a, size_t work_elems, int cu_count)
 {
     using Tile = PagedTile<F16, HDP>;
-    const void *fn = (const void *)paged_attn_kernel<F16, HDP>;
-    const uint32_t hd = a.cache.n[3];
+    const void *fn = (const void *)paged_attn_kernel<F16, HDP, FULL>;
     const size_t lds = (size_t)(a.table.B + 3) / 4 * 16 + Tile::QN * kHeadsPerTile * Tile::QP * (F16 ? 2 : 4) +
-                       4 * kHeadsPerTile * 8 + (size_t)4 * a.tile_heads * hd * 4;
-    static uint64_t done = 0, memo = 0;
+                       4 * kHeadsPerTile * 8 + (size_t)4 * a.tile_heads * a.hd * 4;
+    static uint64_t done = 0;
     const hipError_t e = lds_attr_once(fn, 128 << 10, done);
     if (e != hipSuccess)
         return e;
-    const int per_cu = occupancy_per_cu(fn, 256, lds, memo);
-    if (per_cu <= 0)
-        return hipErrorLaunchFailure;
-    const size_t each = 4 + 2 * part_floats(a.tile_heads, hd); // words of the workspace per workgroup
-    const uint32_t grid = (uint32_t)std::min<size_t>((size_t)per_cu * cu_count, work_elems / each);
+    const size_t want = std::min<size_t>((size_t)Tile::PER_CU * cu_count, kPagedMaxWorkgroups);
+    const uint32_t grid = (uint32_t)std::min(want, work_elems / (4 * part_floats(a.tile_heads, a.hd)));
     if (grid == 0)
         return hipErrorOutOfMemory;
-    a.joins = (uint32_t *)work;
-    a.parts = work + 4 * (size_t)grid;
-    paged_attn_kernel<F16, HDP><<<grid, 256, lds, st>>>(a);
-    paged_join_kernel<F16><<<dim3(grid, a.tile_heads), 256, 0, st>>>(a);
+    paged_attn_kernel<F16, HDP, FULL><<<grid, 256, lds, st>>>(a);
     return hipGetLastError();
 }
 
 hipError_t launch_paged_attn(hipStream_t st, const TView &q, const TView &cache, const PageTableView &table,
                              const TView &out, float scale, const PagedRope &rope, float *work, size_t work_elems,
-                             int cu_count)
+                             uint32_t *arrivals, int cu_count)
 {
-    const uint32_t G = q.n[2] / (cache.n[1] / 2), hd = q.n[3];
-    const float half = cache.dt == DT_F16 && rope.style ? 2.f : 1.f; // the kernel halves rotated fp16 queries
-    PagedAttnArgs a{q, cache, out, table, half * scale * 1.44269504088896340736f, (G - 1) / kHeadsPerTile + 1,
-                    std::min(G, (uint32_t)kHeadsPerTile), nullptr, nullptr, rope};
-    if (cache.dt == DT_F16)
-        return hd <= 64    ? launch_as<true, 64>(st, a, work, work_elems, cu_count)
-               : hd <= 128 ? launch_as<true, 128>(st, a, work, work_elems, cu_count)
-                           : launch_as<true, 256>(st, a, work, work_elems, cu_count);
-    return hd <= 64    ? launch_as<false, 64>(st, a, work, work_elems, cu_count)
-           : hd <= 128 ? launch_as<false, 128>(st, a, work, work_elems, cu_count)
-                       : launch_as<false, 256>(st, a, work, work_elems, cu_count);
+    const uint32_t KV = cache.n[1] / 2, G = q.n[2] / KV, R = cache.n[2], hd = q.n[3], es = cache.dt == DT_F16 ? 2 : 4;
+    PagedAttnArgs a{};
+    a.q = q.p;
+    a.cache = cache.p;
+    a.out = out.p;
+    for (int i = 0; i < 3; ++i)
+    {
+        a.qs[i] = q.s[i + 1];
+        a.os[i] = out.s[i + 1];
+    }
+    a.table = table;
+    a.pages = cache.n[0];
+    a.KV = KV;
+    a.G = G;
+    a.hd = hd;
+    a.page_tiles = R / 16;
+    a.head_bytes = R * hd * es;
+    a.page_bytes = 2 * KV * a.head_bytes;
+    a.groups = (G - 1) / kHeadsPerTile + 1;
+    a.tile_heads = std::min(G, (uint32_t)kHeadsPerTile);
+    // 2^28 * (div_magic * d - 2^div_shift) < 2^28 * d <= 2^div_shift, so the quotient of any t < 2^28 is exact
+    while ((1u << a.div_shift) < a.page_tiles)
+        ++a.div_shift;
+    a.div_shift += 28;
+    a.div_magic = (uint32_t)((((uint64_t)1 << a.div_shift) + a.page_tiles - 1) / a.page_tiles);
+    // the kernel halves rotated fp16 queries
+    a.scale_log2 = (es == 2 && rope.style ? 2.f : 1.f) * scale * 1.44269504088896340736f;
+    a.rope = rope;
+    a.parts = work;
+    a.arrivals = arrivals;
+    const auto run = [&](auto f16) {
+        constexpr bool F16 = decltype(f16)::value;
+        return hd == 64    ? launch_as<F16, 64, true>(st, a, work_elems, cu_count)
+               : hd < 64   ? launch_as<F16, 64, false>(st, a, work_elems, cu_count)
+               : hd == 128 ? launch_as<F16, 128, true>(st, a, work_elems, cu_count)
+               : hd < 128  ? launch_as<F16, 128, false>(st, a, work_elems, cu_count)
+               : hd == 256 ? launch_as<F16, 256, true>(st, a, work_elems, cu_count)
+                           : launch_as<F16, 256, false>(st, a, work_elems, cu_count);
+    };
+    return cache.dt == DT_F16 ? run(std::true_type()) : run(std::false_type());
 }
 
 } // namespace vk

@@ -7,6 +7,13 @@ namespace vk
 
 constexpr uint32_t kNoPage = 0xFFFFFFFFu;
 
+// A word at an address that the whole wave shares and that nothing writes while the kernel runs, as a scalar load: it counts
+// on a counter of its own, so that waiting for it waits for no vector load.
+__device__ __forceinline__ uint32_t scalar_word(const uint32_t *p)
+{
+    return *(const __attribute__((address_space(4))) uint32_t *)(uintptr_t)p;
+}
+
 // (cos, sin) of position * turns full turns. The product is in 64 bits and only its fraction goes on: at position 10^5
 // a 32-bit angle would be off by 2^-8.
 __device__ __forceinline__ float2 turn_at(uint32_t position, double turns)
@@ -17,18 +24,37 @@ __device__ __forceinline__ float2 turn_at(uint32_t position, double turns)
     return r;
 }
 
+template <int ctrl, int row_mask> __device__ __forceinline__ uint64_t dpp_add64(uint64_t v)
+{
+    const uint32_t lo = __builtin_amdgcn_update_dpp(0, (uint32_t)v, ctrl, row_mask, 0xF, false);
+    const uint32_t hi = __builtin_amdgcn_update_dpp(0, (uint32_t)(v >> 32), ctrl, row_mask, 0xF, false);
+    return v + ((uint64_t)hi << 32 | lo);
+}
+
+// sum of `v` over the wave's lanes up to this one
+__device__ __forceinline__ uint64_t wave_scan(uint64_t v)
+{
+    v = dpp_add64<0x111, 0xF>(v); // row_shr:1, 2, 4, 8 within rows of 16
+    v = dpp_add64<0x112, 0xF>(v);
+    v = dpp_add64<0x114, 0xF>(v);
+    v = dpp_add64<0x118, 0xF>(v);
+    v = dpp_add64<0x142, 0xA>(v); // row_bcast:15 -> rows 1, 3
+    v = dpp_add64<0x143, 0xC>(v); // row_bcast:31 -> rows 2, 3
+    return v;
+}
+
+__device__ __forceinline__ uint64_t read_lane(uint64_t v, uint32_t lane)
+{
+    return (uint64_t)(uint32_t)__builtin_amdgcn_readlane((uint32_t)(v >> 32), lane) << 32 |
+           (uint32_t)__builtin_amdgcn_readlane((uint32_t)v, lane);
+}
+
 // Sum of `v` over the threads before this one, and the workgroup's in `total`; `part` holds a word per wave. Every thread
 // calls it; it starts and ends with the workgroup together.
 __device__ __forceinline__ uint64_t block_scan(uint64_t v, uint64_t *part, uint64_t &total)
 {
     const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave, waves = blockDim.x / kWave;
-    uint64_t s = v;
-#pragma unroll
-    for (int o = 1; o < kWave; o <<= 1)
-    {
-        const uint64_t up = __shfl_up((unsigned long long)s, o, kWave);
-        s += lane >= o ? up : 0;
-    }
+    const uint64_t s = wave_scan(v);
     __syncthreads();
     if (lane == kWave - 1)
         part[wave] = s;

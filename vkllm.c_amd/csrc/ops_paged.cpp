@@ -237,6 +237,29 @@ extern "C" vkllm_err_t vkllm_op_update_pages_post_run(struct vkllm_context *, st
 
 // =============================================================================================================
 // PAGED_ATTN
+
+// The context's workspace and arrival counters, made at the first use and kept until the context is freed
+static vkllm_err_t paged_attn_memory(vkllm_context *context, float **work, size_t *work_elems)
+{
+    vkllm_gpu_device *dev = context->device;
+    _CHECK(op_workspace(context, work, work_elems));
+    if (!*work)
+        return VKLLM_ERR_ALLOC;
+    if (dev->paged_arrivals)
+        return VKLLM_ERR_OK;
+    uint32_t *p = nullptr;
+    HIP_TRY(hipMalloc(&p, vk::kPagedArrivals * sizeof(uint32_t)));
+    hipError_t e = hipMemsetAsync(p, 0, vk::kPagedArrivals * sizeof(uint32_t), dev->stream);
+    if (e == hipSuccess)
+        e = hipStreamSynchronize(dev->stream);
+    if (e != hipSuccess)
+    {
+        (void)hipFree(p);
+        return hip_fail(e, "clearing the arrival counters", __FILE__, __LINE__);
+    }
+    dev->paged_arrivals = p;
+    return VKLLM_ERR_OK;
+}
 extern "C" vkllm_err_t vkllm_op_paged_attn_init(struct vkllm_context *context, struct vkllm_commands *commands,
                                                 struct vkllm_tensor *tensor)
 {
@@ -261,9 +284,7 @@ extern "C" vkllm_err_t vkllm_op_paged_attn_init(struct vkllm_context *context, s
     _CHECK_ARGS(std::isfinite(p.scale) && rope_base_ok(p.rope_base));
     float *work = nullptr;
     size_t work_elems = 0;
-    _CHECK(op_workspace(context, &work, &work_elems));
-    if (!work)
-        return VKLLM_ERR_ALLOC;
+    _CHECK(paged_attn_memory(context, &work, &work_elems));
     tensor->pipeline = pipeline_of(context, KID_PAGED_ATTN);
     return VKLLM_ERR_OK;
 }
@@ -286,11 +307,11 @@ extern "C" vkllm_err_t vkllm_op_paged_attn_run(struct vkllm_context *context, st
     NEED_DEV(out);
     float *work = nullptr;
     size_t work_elems = 0;
-    _CHECK(op_workspace(context, &work, &work_elems));
+    _CHECK(paged_attn_memory(context, &work, &work_elems));
     LAUNCH(context, KID_PAGED_ATTN,
            vk::launch_paged_attn(context->device->stream, q, cache, table_view(table), out, p.scale,
                                  rope_of(p.rope_base, p.neox_style, q.n[3]), work, work_elems,
-                                 context->device->cu_count));
+                                 context->device->paged_arrivals, context->device->cu_count));
     commands_note_write(commands, tensor);
     return VKLLM_ERR_OK;
 }

@@ -102,6 +102,8 @@ struct vkllm_gpu_device
     // partial results of the operators that split their work, allocated at the first use (op_workspace)
     float *op_work = nullptr;
     size_t op_work_elems = 0;
+    // the paged attention's arrival counters (launch_paged_attn), zeroed when they are made at the first use
+    uint32_t *paged_arrivals = nullptr;
 };
 
 // ---- errors ----
