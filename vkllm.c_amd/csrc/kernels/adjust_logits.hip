@@ -1,110 +1,232 @@
 // VKLLM_OP_ADJUST_LOGITS: penalties for used tokens, token biases and a grammar's mask. No counterpart in the reference.
 //
-// A workgroup has one tile of one row's vocabulary. It counts the tile's tokens in the row's history and notes their last
-// bias in LDS (whole numbers and a maximum of entry numbers, so the order of the atomics changes nothing), then
-// passes over the logits once. Bound by HBM for batches; every tile of a row reads the row's history again, from L2.
+// A workgroup takes tiles of one row's vocabulary, 32 bytes of logits a thread. It counts the tile's tokens in the row's history and
+// notes their last bias in LDS (whole numbers and a maximum of entry numbers, so the order of the atomics changes
+// nothing), and passes over the logits once, looking every token up. Bound by HBM for batches, by latency for a row.
+// Tiles are as large as still fill the GPU, since each goes through the row's history; a workgroup with several keeps its
+// share of the history in registers and has the next tile's logits on their way while it works on one. 256 rows of 131072
+// fp16 logits, 4096 used tokens, 300 biases and a mask: a tile per workgroup 47 us, 35 now
+// (4.1 TB/s); with nothing to look up 26.
+#include <algorithm>
+
 #include "device_common.h"
+#include "paged_common.h"
 
 namespace vk
 {
+
+constexpr uint32_t kBiasesInLds = 1024;
+constexpr uint32_t kMaxThreads = 1024, kMinThreads = 256, kMinTile = 2048, kWorkgroups = 512;
+// two vectors of logits a thread and tile: with four, fp32 held one workgroup of 1024 threads a CU
+constexpr uint32_t tokens_per_thread(uint32_t size)
+{
+    return 32 / size;
+}
 
 struct AdjustArgs
 {
     TView x, out;
     WordRows history, rules, mask;
     uint32_t tile;
-    bool vec; // rows start on 16-byte boundaries
 };
 
-// dynamic LDS: counts [tile] (if there is a history), last bias entries + 1 [tile] (if there are rules)
-template <typename T> __global__ __launch_bounds__(256) void adjust_logits_kernel(AdjustArgs a)
+struct __attribute__((packed, aligned(4))) Word4
 {
+    u32x4 v;
+};
+// 16 bytes of logits: rows of odd widths start anywhere
+template <typename T, uint32_t N> struct __attribute__((packed, aligned(sizeof(T)))) Logits
+{
+    T v __attribute__((ext_vector_type(N)));
+};
+
+// Dynamic LDS, if there are rules: a word per token of the tile, its count in the low half and the number of its last
+// bias in the high one; WIDE, for histories or biases past 16 bits: a word each.
+template <typename T, bool WIDE> __global__ __launch_bounds__(1024) void adjust_logits_kernel(AdjustArgs a)
+{
+    constexpr uint32_t N = 16 / sizeof(T), VECS = 2;
+    typedef T TN __attribute__((ext_vector_type(N)));
+    typedef Logits<T, N> Vec;
     extern __shared__ uint32_t lds[];
-    const uint32_t t = threadIdx.x, b = blockIdx.y, V = a.x.n[3];
-    const uint32_t v0 = blockIdx.x * a.tile, n = min(a.tile, V - v0);
-    uint32_t *count = lds, *last = a.history.p ? lds + a.tile : lds;
+    __shared__ float values[kBiasesInLds]; // the first biases' values
+    const uint32_t t = threadIdx.x, threads = blockDim.x, b = blockIdx.y, V = a.x.n[3], tile = a.tile;
+    uint32_t *count = lds, *last = WIDE ? lds + tile : lds;
     const uint32_t *rules = a.rules.p ? a.rules.p + (size_t)b * a.rules.stride : nullptr;
-    float rep = 1.f, freq = 0.f, pres = 0.f;
-    if (rules)
-    {
-        const uint32_t n_bias = min(rules[3], (a.rules.n - 4) / 2);
-        rep = __uint_as_float(rules[0]);
-        freq = __uint_as_float(rules[1]);
-        pres = __uint_as_float(rules[2]);
-        for (uint32_t i = t; i < n; i += 256)
+    const uint32_t *mask = a.mask.p ? a.mask.p + (size_t)b * a.mask.stride : nullptr;
+    const T *row = (const T *)a.x.p + (size_t)b * a.x.s[2];
+    T *out = (T *)a.out.p + (size_t)b * a.out.s[2];
+    const uint32_t step = gridDim.x * tile;
+    uint32_t v0 = blockIdx.x * tile;
+    TN y[VECS];
+    uint32_t bits[VECS];
+    auto load = [&](uint32_t v0) {
+#pragma unroll
+        for (uint32_t j = 0; j < VECS; ++j)
         {
-            last[i] = 0;
-            if (a.history.p)
-                count[i] = 0;
-        }
-        __syncthreads();
-        if (a.history.p)
-        {
-            const uint32_t *h = a.history.p + (size_t)b * a.history.stride;
-            const uint32_t used = min(h[0], a.history.n - 1);
-#pragma unroll 4
-            for (uint32_t i = t; i < used; i += 256)
+            const uint32_t v = v0 + (t + j * threads) * N;
+            bits[j] = ~0u;
+            if ((t + j * threads) * N < tile && v + N <= V)
             {
-                const uint32_t v = h[1 + i] - v0;
-                if (v < n)
-                    atomicAdd(&count[v], 1u);
+                y[j] = ((const Vec *)(row + v))->v;
+                if (mask)
+                    bits[j] = mask[v / 32];
             }
         }
-        for (uint32_t i = t; i < n_bias; i += 256)
+    };
+    load(v0);
+    float rep = 1.f, inverse = 1.f, freq = 0.f, pres = 0.f;
+    uint32_t n_bias = 0, used = 0;
+    const uint32_t *h = nullptr;
+    u32x4 mine = {~0u, ~0u, ~0u, ~0u}; // this thread's first part of the history, and its first bias: no token
+    uint32_t my_bias = ~0u;
+    if (rules)
+    {
+        n_bias = min(rules[3], (a.rules.n - 4) / 2);
+        rep = __uint_as_float(rules[0]);
+        inverse = 1.f / rep; // a product instead of a division per token: off by one roundoff of 32 bits more
+        freq = __uint_as_float(rules[1]);
+        pres = __uint_as_float(rules[2]);
+        if (a.history.p)
         {
-            const uint32_t v = rules[4 + 2 * i] - v0;
-            if (v < n)
-                atomicMax(&last[v], i + 1);
+            h = a.history.p + (size_t)b * a.history.stride + 1;
+            used = min(h[-1], a.history.n - 1);
+            if (t < used / 4)
+                mine = ((const Word4 *)h)[t].v;
         }
-        __syncthreads();
+        if (t < n_bias)
+            my_bias = rules[4 + 2 * t];
+        for (uint32_t i = t; i < min(n_bias, kBiasesInLds); i += threads)
+            values[i] = __uint_as_float(rules[5 + 2 * i]);
+        for (uint32_t i = t; i < (WIDE ? 2 : 1) * tile / 4; i += threads)
+            ((u32x4 *)lds)[i] = (u32x4){0, 0, 0, 0};
     }
-    const uint32_t *mask = a.mask.p ? a.mask.p + (size_t)b * a.mask.stride : nullptr;
-    const T *x = (const T *)a.x.p + (size_t)b * a.x.s[2] + v0;
-    T *out = (T *)a.out.p + (size_t)b * a.out.s[2] + v0;
-    auto adjust = [&](float y, uint32_t v, bool allowed) {
+    auto bias_of = [&](uint32_t entry) {
+        return entry <= kBiasesInLds ? values[entry - 1] : __uint_as_float(rules[5 + 2 * (entry - 1)]);
+    };
+    // the logit of token v0 + v
+    auto adjusted = [&](float y, uint32_t v) {
+        const uint32_t c = WIDE ? count[v] : count[v] & 0xFFFFu, e = WIDE ? last[v] : last[v] >> 16;
+        const float p = (y > 0.f ? y * inverse : y * rep) - (freq * (float)c + pres);
+        y = c ? p : y;
+        return e ? y + bias_of(e) : y;
+    };
+    for (; v0 < V; v0 += step)
+    {
+        const uint32_t n = min(tile, V - v0), nv = n / N;
         if (rules)
         {
-            const uint32_t c = a.history.p ? count[v] : 0;
-            if (c)
-                y = (y > 0.f ? y / rep : y * rep) - (freq * (float)c + pres);
-            if (last[v])
-                y += __uint_as_float(rules[5 + 2 * (last[v] - 1)]);
-        }
-        return (T)(allowed ? y : -INFINITY);
-    };
-    constexpr uint32_t N = 16 / sizeof(T);
-    typedef T TN __attribute__((ext_vector_type(N)));
-    const uint32_t nv = a.vec ? n / N : 0;
-    for (uint32_t i = t; i < nv; i += 256)
-    {
-        TN y = *(const TN *)(x + i * N);
-        const uint32_t bits = mask ? mask[(v0 + i * N) / 32] >> ((v0 + i * N) % 32) : ~0u;
+            lds_barrier(); // the words are zero
+            auto note = [&](uint32_t token) {
+                if (token - v0 < n)
+                    atomicAdd(&count[token - v0], 1u);
+            };
 #pragma unroll
-        for (uint32_t k = 0; k < N; ++k)
-            y[k] = adjust((float)y[k], i * N + k, (bits >> k) & 1);
-        *(TN *)(out + i * N) = y;
+            for (int k = 0; k < 4; ++k)
+                note(mine[k]);
+            for (uint32_t i = t + threads; i < used / 4; i += threads)
+            {
+                const u32x4 w = ((const Word4 *)h)[i].v;
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                    note(w[k]);
+            }
+            if (t < used % 4)
+                note(h[used / 4 * 4 + t]);
+            lds_barrier();
+            for (uint32_t i = t; i < n_bias; i += threads)
+            {
+                const uint32_t v = (i == t ? my_bias : rules[4 + 2 * i]) - v0;
+                if (v < n) // the counts stand, so the largest word is that of the last entry
+                    atomicMax(&last[v], WIDE ? i + 1 : (i + 1) << 16 | (count[v] & 0xFFFFu));
+            }
+            lds_barrier();
+        }
+        TN z[VECS];
+        uint32_t ok[VECS];
+#pragma unroll
+        for (uint32_t j = 0; j < VECS; ++j)
+        {
+            z[j] = y[j];
+            ok[j] = bits[j] >> ((v0 + (t + j * threads) * N) % 32);
+        }
+        if (v0 + step < V)
+            load(v0 + step);
+#pragma unroll
+        for (uint32_t j = 0; j < VECS; ++j)
+        {
+            const uint32_t v = (t + j * threads) * N;
+            if (t + j * threads >= nv)
+                continue;
+            if (rules)
+            {
+                u32x4 w[N / 4], any = {0, 0, 0, 0};
+#pragma unroll
+                for (uint32_t k = 0; k < N / 4; ++k)
+                {
+                    w[k] = *(const u32x4 *)(count + v + 4 * k);
+                    any |= w[k];
+                    if (WIDE)
+                        any |= *(const u32x4 *)(last + v + 4 * k);
+                }
+                if (any[0] | any[1] | any[2] | any[3])
+                {
+#pragma unroll
+                    for (uint32_t k = 0; k < N; ++k)
+                        z[j][k] = (T)adjusted((float)z[j][k], v + k);
+#pragma unroll
+                    for (uint32_t k = 0; k < N / 4; ++k)
+                    {
+                        *(u32x4 *)(count + v + 4 * k) = (u32x4){0, 0, 0, 0};
+                        if (WIDE)
+                            *(u32x4 *)(last + v + 4 * k) = (u32x4){0, 0, 0, 0};
+                    }
+                }
+            }
+#pragma unroll
+            for (uint32_t k = 0; k < N; ++k)
+                z[j][k] = (ok[j] >> k) & 1 ? z[j][k] : (T)-INFINITY;
+            ((Vec *)(out + v0 + v))->v = z[j];
+        }
+        for (uint32_t v = nv * N + t; v < n; v += threads)
+        {
+            float y = (float)row[v0 + v];
+            if (rules)
+            {
+                y = adjusted(y, v);
+                count[v] = 0;
+                last[v] = 0;
+            }
+            out[v0 + v] = !mask || (mask[(v0 + v) / 32] >> ((v0 + v) % 32)) & 1 ? (T)y : (T)-INFINITY;
+        }
     }
-    for (uint32_t i = nv * N + t; i < n; i += 256)
-        out[i] = adjust((float)x[i], i, !mask || (mask[(v0 + i) / 32] >> ((v0 + i) % 32)) & 1);
+}
+
+template <typename T, bool WIDE> static hipError_t launch_as(hipStream_t st, const AdjustArgs &a)
+{
+    const uint32_t threads = std::max(a.tile / tokens_per_thread(sizeof(T)), kMinThreads), V = a.x.n[3], B = a.x.n[2];
+    const size_t lds = a.rules.p ? (WIDE ? 8 : 4) * (size_t)a.tile : 0;
+    static uint64_t done = 0;
+    const hipError_t e = lds_attr_once((const void *)adjust_logits_kernel<T, WIDE>, 8 * kMaxThreads * tokens_per_thread(sizeof(T)), done);
+    if (e != hipSuccess)
+        return e;
+    const uint32_t tiles = (V - 1) / a.tile + 1;
+    const uint32_t groups = std::min(tiles, (kWorkgroups - 1) / B + 1);
+    adjust_logits_kernel<T, WIDE><<<dim3(groups, B), threads, lds, st>>>(a);
+    return hipGetLastError();
 }
 
 hipError_t launch_adjust_logits(hipStream_t st, const TView &x, const TView &out, const WordRows &history,
                                 const WordRows &rules, const WordRows &mask)
 {
-    const uint32_t B = x.n[2], V = x.n[3], N = x.dt == DT_F16 ? 8 : 4;
-    auto vec = [N](const TView &t) { return (t.n[2] == 1 || t.s[2] % N == 0) && (uintptr_t)t.p % 16 == 0; };
-    // whole mask words per tile; small batches take small tiles, so that the GPU is filled
-    uint32_t tile = 8192;
-    while (tile > 1024 && (uint64_t)B * ((V - 1) / tile + 1) < 512)
+    const uint32_t B = x.n[2], V = x.n[3];
+    uint32_t tile = kMaxThreads * tokens_per_thread(x.dt == DT_F16 ? 2 : 4); // whole mask words per tile
+    while (tile > kMinTile && (uint64_t)B * ((V - 1) / tile + 1) < kWorkgroups)
         tile /= 2;
-    const AdjustArgs a{x, out, history, rules, mask, tile, vec(x) && vec(out)};
-    const size_t lds = rules.p ? (history.p ? 8 : 4) * (size_t)tile : 0;
-    const dim3 grid((V - 1) / tile + 1, B);
+    const AdjustArgs a{x, out, history, rules, mask, tile};
+    const bool wide = std::max(history.n, rules.n) > 65535;
     if (x.dt == DT_F16)
-        adjust_logits_kernel<_Float16><<<grid, 256, lds, st>>>(a);
-    else
-        adjust_logits_kernel<float><<<grid, 256, lds, st>>>(a);
-    return hipGetLastError();
+        return wide ? launch_as<_Float16, true>(st, a) : launch_as<_Float16, false>(st, a);
+    return wide ? launch_as<float, true>(st, a) : launch_as<float, false>(st, a);
 }
 
 } // namespace vk

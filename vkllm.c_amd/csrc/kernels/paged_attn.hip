@@ -101,12 +101,6 @@ __device__ __forceinline__ float exp2_of(float x)
     return __builtin_amdgcn_exp2f(x);
 }
 
-// the workgroup meets; what it wrote to LDS is seen. Loads from memory stay in flight, which __syncthreads would wait for.
-__device__ __forceinline__ void lds_barrier()
-{
-    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-}
-
 // dynamic LDS: lengths [B], queries [QN][16][QP], per-wave statistics [4][16][2], per-wave sums [4][tile_heads][hd]
 // FULL: head_dim is HDP, else it is smaller
 template <bool F16, int HDP, bool FULL>

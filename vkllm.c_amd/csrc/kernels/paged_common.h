@@ -7,6 +7,12 @@ namespace vk
 
 constexpr uint32_t kNoPage = 0xFFFFFFFFu;
 
+// the workgroup meets; what it wrote to LDS is seen. Loads from memory stay in flight, which __syncthreads would wait for.
+__device__ __forceinline__ void lds_barrier()
+{
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+}
+
 // A word at an address that the whole wave shares and that nothing writes while the kernel runs, as a scalar load: it counts
 // on a counter of its own, so that waiting for it waits for no vector load.
 __device__ __forceinline__ uint32_t scalar_word(const uint32_t *p)
