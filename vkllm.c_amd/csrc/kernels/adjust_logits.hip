@@ -30,10 +30,6 @@ struct AdjustArgs
     uint32_t tile;
 };
 
-struct __attribute__((packed, aligned(4))) Word4
-{
-    u32x4 v;
-};
 // 16 bytes of logits: rows of odd widths start anywhere
 template <typename T, uint32_t N> struct __attribute__((packed, aligned(sizeof(T)))) Logits
 {

@@ -55,9 +55,11 @@ struct PageTableView
     uint32_t *p;
     uint32_t B, P, stride;
 };
-// want [B] with element stride want_s; old: the table so far, or nullptr to bring `out` up to date in place
+// want [B] with element stride want_s; old: the table so far, or nullptr to bring `out` up to date in place; work
+// (work_elems words, 8-byte aligned) and one arrival counter, zero before and after, for a launch of several marking workgroups
 hipError_t launch_page_table(hipStream_t st, const PageTableView &out, const uint32_t *old, uint32_t old_stride,
-                             const uint32_t *want, uint32_t want_s, uint32_t page_rows, uint32_t pages, int cu_count);
+                             const uint32_t *want, uint32_t want_s, uint32_t page_rows, uint32_t pages, float *work,
+                             size_t work_elems, uint32_t *arrivals, int cu_count);
 // map [T] pairs (slot, position), packed
 hipError_t launch_slot_map(hipStream_t st, const PageTableView &table, const uint32_t *lengths, uint32_t lengths_s,
                            const uint32_t *counts, uint32_t counts_s, uint32_t *map, uint32_t T, uint32_t page_rows);

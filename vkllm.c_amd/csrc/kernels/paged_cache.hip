@@ -1,5 +1,7 @@
 // The page table of a batch, the slot map of a step's new tokens, and the writes into a paged cache
 // (VKLLM_OP_PAGE_TABLE, SLOT_MAP, UPDATE_PAGES). No counterpart in the reference.
+#include <algorithm>
+
 #include "device_common.h"
 #include "paged_common.h"
 
@@ -12,11 +14,13 @@ namespace vk
 // it; the k-th free page goes to the row whose demand, summed in row order, covers k. Rows whose sum passes
 // the number of free pages keep what they had.
 //
-// Workgroup 0 does that: bits and prefix sums stand in its LDS, so the table is built in one launch without an
-// exchange between workgroups. It writes the lengths and the columns [keep, keep + need). The others write
-// the remaining columns, which hang on a row's own lengths only: the kept ids (unless in place) and NO_PAGE behind.
+// The first `markers` workgroups mark the kept pages, each those of its share of the rows, in bits in LDS. The last of them to
+// arrive (none waits) takes the others' bits from the workspace, and has the prefix sums, the free list and the lengths in its
+// own LDS: it writes the lengths and the columns [keep, keep + need). The other workgroups write the remaining columns,
+// which hang on a row's own lengths only: the kept ids (unless in place) and NO_PAGE behind. One launch. Bound by latency
+// and by a CU's rate of LDS atomics: 256 rows of up to 512 pages of 65536 take 11.8 us, 16.8 with one marking workgroup;
+// 1000 rows of up to 700 of 400000 with slots and positions of 8000 tokens 33 us, 58 with five.
 constexpr int kTableThreads = 1024;
-constexpr uint32_t kListLen = 4096; // free pages handed out at a time
 
 struct PageTableArgs
 {
@@ -25,7 +29,12 @@ struct PageTableArgs
     uint32_t old_stride;
     const uint32_t *want;
     uint32_t want_s, R, pages;
+    uint32_t markers;
+    uint32_t *bits;     // [markers][bits of all pages], even numbers of words
+    uint32_t *arrivals; // zero between launches
 };
+constexpr uint32_t kMarkColumns = 256; // columns of a row that a wave marks at once
+constexpr uint32_t kMarkPieces = 32, kMaxMarkers = 16;
 
 __device__ __forceinline__ uint32_t ceil_pages(uint32_t len, uint32_t R)
 {
@@ -49,10 +58,10 @@ __global__ __launch_bounds__(kTableThreads) void page_table_kernel(PageTableArgs
 {
     extern __shared__ uint32_t lds[];
     const uint32_t t = threadIdx.x, B = a.out.B, P = a.out.P, R = a.R;
-    if (blockIdx.x > 0)
+    if (blockIdx.x >= a.markers)
     {
-        // the columns of rows b, b + gridDim.x - 1, ...: a thread per column
-        for (uint32_t b = blockIdx.x - 1; b < B; b += gridDim.x - 1)
+        // the columns of rows b, b + (such workgroups), ...: a thread per column
+        for (uint32_t b = blockIdx.x - a.markers; b < B; b += gridDim.x - a.markers)
         {
             const uint32_t want = a.want[(size_t)b * a.want_s];
             uint32_t *to = a.out.p + (size_t)b * a.out.stride + 1;
@@ -70,13 +79,15 @@ __global__ __launch_bounds__(kTableThreads) void page_table_kernel(PageTableArgs
         }
         return;
     }
-    const uint32_t words = (a.pages + 31) / 32;
-    uint32_t *used = lds, *start = used + words, *keeps = start + B + 1, *list = keeps + B;
+    const uint32_t words = (a.pages + 63) / 64 * 2;
+    uint32_t *used = lds, *start = used + words, *keeps = start + B + 1, *hads = keeps + B, *wants = hads + B,
+             *ranks = wants + B;
     __shared__ uint64_t scan[kTableThreads / kWave];
+    __shared__ uint32_t arrived;
     const uint32_t *old = a.old ? a.old : a.out.p;
     const uint32_t old_stride = a.old ? a.old_stride : a.out.stride;
     for (uint32_t w = t; w < words; w += kTableThreads) // bits past the last page count as used
-        used[w] = w * 32 + 32 <= a.pages ? 0u : ~0u << (a.pages % 32);
+        used[w] = w * 32 + 32 <= a.pages ? 0u : w * 32 >= a.pages ? ~0u : ~0u << (a.pages % 32);
     // demands, summed in row order: thread t has rows t * per .. t * per + per - 1
     const uint32_t per = (B + kTableThreads - 1) / kTableThreads;
     uint64_t mine = 0;
@@ -84,43 +95,80 @@ __global__ __launch_bounds__(kTableThreads) void page_table_kernel(PageTableArgs
     {
         const RowPages r = row_pages(old[(size_t)b * old_stride], a.want[(size_t)b * a.want_s], R, P);
         keeps[b] = r.keep;
+        hads[b] = r.had;
+        wants[b] = r.want;
+        start[b] = r.need;
         mine += r.need;
     }
     uint64_t total;
     uint64_t at = block_scan(mine, scan, total);
     for (uint32_t b = t * per; b < t * per + per && b < B; ++b)
     {
-        const RowPages r = row_pages(old[(size_t)b * old_stride], a.want[(size_t)b * a.want_s], R, P);
-        start[b] = (uint32_t)at; // sums past 32 bits are past the last page, too (below)
-        at += r.need;
+        const uint32_t need = start[b];
+        start[b] = (uint32_t)at; // a table has fewer than 2^30 columns in all
+        at += need;
     }
     if (t == 0)
         start[B] = (uint32_t)total;
     __syncthreads();
-    // mark the kept pages: a wave takes 8 rows at a time, so that 8 reads are in flight
-    const uint32_t lane = t % kWave, wave = t / kWave, waves = kTableThreads / kWave;
-    for (uint32_t b0 = wave * 8; b0 < B; b0 += waves * 8)
+    // Marks: a wave takes 256 columns of 4 rows at a time, neighbouring lanes neighbouring columns, 16 ids a lane on their way
+    const uint32_t lane = t % kWave, wave = __builtin_amdgcn_readfirstlane(t / kWave), waves = kTableThreads / kWave;
+    const uint32_t chunks = (P - 1) / kMarkColumns + 1, rows = (B - 1) / a.markers + 1, first = blockIdx.x * rows;
+    const uint32_t items = first < B ? min(rows, B - first) * chunks : 0;
+    for (uint32_t i0 = wave * 4; i0 < items; i0 += waves * 4)
     {
-        uint32_t most = 0;
+        uint32_t id[4][4], keep[4], c[4];
 #pragma unroll
-        for (uint32_t i = 0; i < 8; ++i)
-            most = max(most, b0 + i < B ? keeps[b0 + i] : 0u);
-        for (uint32_t c = lane; c < most; c += kWave)
+        for (uint32_t i = 0; i < 4; ++i)
         {
-            uint32_t id[8];
+            // columns past the kept ones repeat the last, so that no load is conditional
+            const uint32_t item = min(i0 + i, items - 1), b = first + item / chunks;
+            const uint32_t *row = old + (size_t)b * old_stride;
+            c[i] = item % chunks * kMarkColumns;
+            keep[i] = __builtin_amdgcn_readfirstlane(keeps[b]);
 #pragma unroll
-            for (uint32_t i = 0; i < 8; ++i)
-            {
-                const uint32_t b = min(b0 + i, B - 1);
-                id[i] = b0 + i < B && c < keeps[b] ? old[(size_t)b * old_stride + 1 + c] : kNoPage;
-            }
-#pragma unroll
-            for (uint32_t i = 0; i < 8; ++i)
-                if (id[i] < a.pages)
-                    atomicOr(&used[id[i] / 32], 1u << (id[i] % 32));
+            for (uint32_t k = 0; k < 4; ++k)
+                id[i][k] = row[min(1 + c[i] + k * kWave + lane, keep[i])];
         }
+        // all are asked for before the first is looked at (the compiler would move each load to its use)
+#pragma unroll
+        for (uint32_t i = 0; i < 4; ++i)
+            asm volatile("" : "+v"(id[i][0]), "+v"(id[i][1]), "+v"(id[i][2]), "+v"(id[i][3]));
+#pragma unroll
+        for (uint32_t i = 0; i < 4; ++i)
+#pragma unroll
+            for (uint32_t k = 0; k < 4; ++k)
+                if (c[i] + k * kWave + lane < keep[i] && id[i][k] < a.pages)
+                    atomicOr(&used[id[i][k] / 32], 1u << (id[i][k] % 32));
     }
     __syncthreads();
+    if (a.markers > 1)
+    {
+        uint64_t *bits = (uint64_t *)a.bits;
+        const uint64_t *mine = (const uint64_t *)used;
+        for (uint32_t w = t; w < words / 2; w += kTableThreads)
+            __hip_atomic_store(bits + (size_t)blockIdx.x * (words / 2) + w, mine[w], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        __builtin_amdgcn_s_waitcnt(0); // this thread's bits are there
+        __syncthreads();
+        if (t == 0)
+        {
+            arrived = __hip_atomic_fetch_add(a.arrivals, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            if (arrived == a.markers - 1)
+                __hip_atomic_store(a.arrivals, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); // for the next launch
+        }
+        __syncthreads();
+        if (arrived != a.markers - 1)
+            return;
+        for (uint32_t w = t; w < words / 2; w += kTableThreads)
+        {
+            uint64_t any = mine[w];
+#pragma unroll 8
+            for (uint32_t g = 0; g < a.markers; ++g)
+                any |= __hip_atomic_load(bits + (size_t)g * (words / 2) + w, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            ((uint64_t *)used)[w] = any;
+        }
+        __syncthreads();
+    }
     // free pages before thread t's words
     const uint32_t wper = (words + kTableThreads - 1) / kTableThreads;
     uint64_t free_mine = 0;
@@ -128,52 +176,62 @@ __global__ __launch_bounds__(kTableThreads) void page_table_kernel(PageTableArgs
         free_mine += __popc(~used[w]);
     uint64_t nfree;
     const uint64_t rank0 = block_scan(free_mine, scan, nfree);
-    // the rows that fit: a demand of total pages ends at min(total, nfree) of the list
+    ranks[t] = (uint32_t)rank0;
+    __syncthreads();
+    // The k-th free page to the row with start[b] <= k < start[b + 1], a thread per k: the page is found from the ranks of the
+    // threads' words, counts of bits and halves of a word
     const uint32_t last = (uint32_t)(total < nfree ? total : nfree);
-    for (uint32_t base = 0; base < last; base += kListLen)
+    for (uint32_t k = t; k < last; k += kTableThreads)
     {
-        uint64_t rank = rank0;
-        for (uint32_t w = t * wper; w < t * wper + wper && w < words && rank < (uint64_t)base + kListLen; ++w)
-            for (uint32_t m = ~used[w]; m; m &= m - 1, ++rank)
-                if (rank >= base && rank < (uint64_t)base + kListLen)
-                    list[rank - base] = w * 32 + __ffs(m) - 1;
-        __syncthreads();
-        const uint32_t n = min(kListLen, last - base);
-        for (uint32_t i = t; i < n; i += kTableThreads)
+        const uint32_t owner = last_at_most(ranks, kTableThreads, k);
+        uint32_t w = owner * wper, nth = k - ranks[owner], at = 0;
+        for (; nth >= (uint32_t)__popc(~used[w]); ++w)
+            nth -= __popc(~used[w]);
+        uint32_t bits = ~used[w];
+#pragma unroll
+        for (uint32_t half = 16; half > 0; half /= 2)
         {
-            // the row with start[b] <= k < start[b + 1]: the last whose start is at most k (rows without demand before it
-            // have the same start)
-            const uint32_t k = base + i, b = last_at_most(start, B, k);
-            const uint32_t need = start[b + 1] - start[b];
-            if ((uint64_t)start[b] + need <= nfree)
-                a.out.p[(size_t)b * a.out.stride + 1 + keeps[b] + (k - start[b])] = list[i];
+            const uint32_t below = __popc(bits & ((1u << half) - 1));
+            const bool up = nth >= below;
+            nth -= up ? below : 0;
+            at += up ? half : 0;
+            bits = up ? bits >> half : bits;
         }
-        __syncthreads();
+        // the last row whose start is at most k (rows without demand before it have the same start)
+        const uint32_t b = last_at_most(start, B, k), need = start[b + 1] - start[b];
+        if ((uint64_t)start[b] + need <= nfree)
+            a.out.p[(size_t)b * a.out.stride + 1 + keeps[b] + (k - start[b])] = w * 32 + at;
     }
     // lengths, and NO_PAGE where a row that does not fit would have had its pages
     for (uint32_t b = t; b < B; b += kTableThreads)
     {
-        const RowPages r = row_pages(old[(size_t)b * old_stride], a.want[(size_t)b * a.want_s], R, P);
-        const bool fits = r.need == 0 || (uint64_t)start[b] + r.need <= nfree;
+        const uint32_t need = start[b + 1] - start[b];
+        const bool fits = need == 0 || (uint64_t)start[b] + need <= nfree;
         uint32_t *row = a.out.p + (size_t)b * a.out.stride;
         if (!fits)
-            for (uint32_t c = 0; c < r.need; ++c)
-                row[1 + r.keep + c] = kNoPage;
-        row[0] = fits ? r.want : r.had;
+            for (uint32_t c = 0; c < need; ++c)
+                row[1 + keeps[b] + c] = kNoPage;
+        row[0] = fits ? wants[b] : hads[b];
     }
 }
 
 hipError_t launch_page_table(hipStream_t st, const PageTableView &out, const uint32_t *old, uint32_t old_stride,
-                             const uint32_t *want, uint32_t want_s, uint32_t page_rows, uint32_t pages, int cu_count)
+                             const uint32_t *want, uint32_t want_s, uint32_t page_rows, uint32_t pages, float *work,
+                             size_t work_elems, uint32_t *arrivals, int cu_count)
 {
-    const size_t lds = ((pages + 31) / 32 + 2 * (size_t)out.B + 1 + kListLen) * 4;
+    const uint32_t words = (pages + 63) / 64 * 2;
+    const size_t lds = (words + 4 * (size_t)out.B + 1 + kTableThreads) * 4; // 132 KB at most
     static uint64_t done = 0;
-    const hipError_t e = lds_attr_once((const void *)page_table_kernel, 128 << 10, done);
+    const hipError_t e = lds_attr_once((const void *)page_table_kernel, 134 << 10, done);
     if (e != hipSuccess)
         return e;
-    const uint32_t fill = min(out.B, (uint32_t)cu_count);
-    page_table_kernel<<<1 + fill, kTableThreads, lds, st>>>(
-        PageTableArgs{out, old, old_stride, want, want_s, page_rows, pages});
+    // at least kMarkPieces pieces of 256 columns to a marking workgroup, and at most 1 MB of bits for the last to read
+    const uint64_t pieces = (uint64_t)out.B * ((out.P - 1) / kMarkColumns + 1);
+    const uint32_t markers = (uint32_t)std::max<uint64_t>(
+        1, std::min<uint64_t>({out.B, pieces / kMarkPieces, kMaxMarkers, (256 << 10) / words, work_elems / words}));
+    const uint32_t fill = std::min(out.B, (uint32_t)cu_count);
+    page_table_kernel<<<markers + fill, kTableThreads, lds, st>>>(PageTableArgs{
+        out, old, old_stride, want, want_s, page_rows, pages, markers, (uint32_t *)work, arrivals});
     return hipGetLastError();
 }
 
@@ -184,17 +242,25 @@ __global__ __launch_bounds__(256) void slot_map_kernel(PageTableView table, cons
                                                        const uint32_t *counts, uint32_t counts_s, uint2 *map,
                                                        uint32_t T, uint32_t R)
 {
-    extern __shared__ uint32_t start[]; // [B + 1], sums that end at T
+    extern __shared__ uint32_t start[]; // [B + 1], sums that end at T; then the rows' lengths, counts and held positions
     __shared__ uint64_t scan[4];
     const uint32_t t = threadIdx.x, B = table.B, per = (B + 255) / 256;
+    uint32_t *length = start + B + 1, *count = length + B, *held = count + B;
+    const uint64_t most = (uint64_t)table.P * R;
     uint64_t mine = 0, total;
     for (uint32_t b = t * per; b < t * per + per && b < B; ++b)
-        mine += counts[(size_t)b * counts_s];
+    {
+        const uint32_t len = table.p[(size_t)b * table.stride];
+        held[b] = len > most ? (uint32_t)most : len;
+        length[b] = lengths[(size_t)b * lengths_s];
+        count[b] = counts[(size_t)b * counts_s];
+        mine += count[b];
+    }
     uint64_t at = block_scan(mine, scan, total);
     for (uint32_t b = t * per; b < t * per + per && b < B; ++b)
     {
         start[b] = (uint32_t)min(at, (uint64_t)T);
-        at += counts[(size_t)b * counts_s];
+        at += count[b];
     }
     if (t == 0)
         start[B] = (uint32_t)min(total, (uint64_t)T);
@@ -206,14 +272,12 @@ __global__ __launch_bounds__(256) void slot_map_kernel(PageTableView table, cons
     if (i < start[B])
     {
         const uint32_t b = last_at_most(start, B, i);
-        const uint32_t *row = table.p + (size_t)b * table.stride;
-        const uint64_t most = (uint64_t)table.P * R;
-        const uint32_t len = row[0] > most ? (uint32_t)most : row[0];
-        // a count over the length puts the position below 0, past every length in 32 bits or not held all the same
-        const int64_t pos = (int64_t)lengths[(size_t)b * lengths_s] - counts[(size_t)b * counts_s] + (i - start[b]);
-        if (pos >= 0 && pos < len)
+        // a count over the length puts the position below 0
+        const int64_t pos = (int64_t)length[b] - count[b] + (i - start[b]);
+        if (pos >= 0 && pos < held[b])
         {
-            const uint64_t slot = (uint64_t)row[1 + (uint32_t)pos / R] * R + (uint32_t)pos % R;
+            const uint32_t page = table.p[(size_t)b * table.stride + 1 + (uint32_t)pos / R];
+            const uint64_t slot = (uint64_t)page * R + (uint32_t)pos % R;
             if (slot < kNoPage)
                 out = {(uint32_t)slot, (uint32_t)pos};
         }
@@ -224,51 +288,56 @@ __global__ __launch_bounds__(256) void slot_map_kernel(PageTableView table, cons
 hipError_t launch_slot_map(hipStream_t st, const PageTableView &table, const uint32_t *lengths, uint32_t lengths_s,
                            const uint32_t *counts, uint32_t counts_s, uint32_t *map, uint32_t T, uint32_t page_rows)
 {
-    slot_map_kernel<<<(T - 1) / 256 + 1, 256, ((size_t)table.B + 1) * 4, st>>>(table, lengths, lengths_s, counts,
+    static uint64_t done = 0;
+    const hipError_t e = lds_attr_once((const void *)slot_map_kernel, (4 * kPagedMaxRows + 1) * 4, done);
+    if (e != hipSuccess)
+        return e;
+    slot_map_kernel<<<(T - 1) / 256 + 1, 256, (4 * (size_t)table.B + 1) * 4, st>>>(table, lengths, lengths_s, counts,
                                                                                counts_s, (uint2 *)map, T, page_rows);
     return hipGetLastError();
 }
 
 // ---------------------------------------------------------------------------------------------------------------
 // VKLLM_OP_UPDATE_PAGES. A workgroup has one token (or a share of its heads): the rotations of its position go
-// into LDS once, then a thread moves units of 8 elements of a head: elements 8u .. 8u + 7, or for pairs of halves
-// 4u .. 4u + 3 and as many behind the half. Bound by HBM for prompts, by latency for a token.
+// into LDS once, then a thread moves units of a head: neighbouring elements, or for pairs of halves as many of both. Bound by HBM for prompts, by latency for a token.
 struct UpdatePagesArgs
 {
     TView cache, k, v;
     const uint32_t *map;
     uint32_t map_s;
-    uint32_t units; // of a share: 2 KV heads x hd / 8 over gridDim.y shares
+    uint32_t units; // of a share: those of 2 KV heads over gridDim.y shares
     bool vec;       // k and v rows are contiguous and start on 16-byte boundaries
     PagedRope rope;
 };
 
-template <typename T> __device__ __forceinline__ void load4(const T *p, size_t stride, bool vec, float x[4])
+// N neighbouring elements in 32 bits
+template <typename T, int N> __device__ __forceinline__ void load_n(const T *p, size_t stride, bool vec, float x[N])
 {
-    typedef T T4 __attribute__((ext_vector_type(4)));
+    typedef T TN __attribute__((ext_vector_type(N)));
     if (vec)
     {
-        const T4 v = *(const T4 *)p;
+        const TN v = *(const TN *)p;
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
+        for (int i = 0; i < N; ++i)
             x[i] = (float)v[i];
         return;
     }
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int i = 0; i < N; ++i)
         x[i] = (float)p[i * stride];
 }
-template <typename T> __device__ __forceinline__ void store4(T *p, const float x[4])
+template <typename T, int N> __device__ __forceinline__ void store_n(T *p, const float x[N])
 {
-    typedef T T4 __attribute__((ext_vector_type(4)));
-    T4 v;
+    typedef T TN __attribute__((ext_vector_type(N)));
+    TN v;
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int i = 0; i < N; ++i)
         v[i] = (T)x[i];
-    *(T4 *)p = v;
+    *(TN *)p = v;
 }
 
-template <typename T> __global__ __launch_bounds__(256) void update_pages_kernel(UpdatePagesArgs a)
+// HALF: how many elements of each half of a head a thread takes for pairs of halves; 2 HALF neighbouring ones otherwise
+template <typename T, int HALF> __global__ __launch_bounds__(256) void update_pages_kernel(UpdatePagesArgs a)
 {
     __shared__ float2 cs[kPagedMaxHd / 2];
     const uint32_t tok = blockIdx.x, t = threadIdx.x;
@@ -283,7 +352,7 @@ template <typename T> __global__ __launch_bounds__(256) void update_pages_kernel
             cs[t] = turn_at(pos, a.rope.turns[t]);
         __syncthreads();
     }
-    const uint32_t per = hd / 8, all = 2 * KV * per;
+    const uint32_t per = hd / (2 * HALF), all = 2 * KV * per;
     T *to = (T *)a.cache.p + (size_t)page * a.cache.s[0] + (size_t)(slot % R) * hd;
     for (uint32_t u = blockIdx.y * a.units + t; u < min(all, (blockIdx.y + 1) * a.units); u += 256)
     {
@@ -292,16 +361,16 @@ template <typename T> __global__ __launch_bounds__(256) void update_pages_kernel
         const T *from = (const T *)src.p + (size_t)tok * src.s[1] + (size_t)(h < KV ? h : h - KV) * src.s[2];
         T *row = to + (size_t)h * a.cache.s[1];
         const bool halves = style == 2 && h < KV;
-        const uint32_t d0 = halves ? 4 * c : 8 * c, d1 = halves ? hd / 2 + 4 * c : 8 * c + 4;
-        float x[4], y[4];
-        load4(from + (size_t)d0 * src.s[3], src.s[3], a.vec, x);
-        load4(from + (size_t)d1 * src.s[3], src.s[3], a.vec, y);
+        const uint32_t d0 = HALF * (halves ? c : 2 * c), d1 = d0 + (halves ? hd / 2 : HALF);
+        float x[HALF], y[HALF];
+        load_n<T, HALF>(from + (size_t)d0 * src.s[3], src.s[3], a.vec, x);
+        load_n<T, HALF>(from + (size_t)d1 * src.s[3], src.s[3], a.vec, y);
         if (halves)
         {
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
+            for (int i = 0; i < HALF; ++i)
             {
-                const float2 r = cs[4 * c + i];
+                const float2 r = cs[d0 + i];
                 const float p = x[i], q = y[i];
                 x[i] = r.x * p - r.y * q;
                 y[i] = r.y * p + r.x * q;
@@ -309,21 +378,21 @@ template <typename T> __global__ __launch_bounds__(256) void update_pages_kernel
         }
         else if (style && h < KV)
         {
+            auto turn = [&](float *v, uint32_t w) {
 #pragma unroll
-            for (int i = 0; i < 2; ++i)
-            {
-                const float2 r = cs[4 * c + i], s = cs[4 * c + 2 + i];
-                float p = x[2 * i], q = x[2 * i + 1];
-                x[2 * i] = r.x * p - r.y * q;
-                x[2 * i + 1] = r.y * p + r.x * q;
-                p = y[2 * i];
-                q = y[2 * i + 1];
-                y[2 * i] = s.x * p - s.y * q;
-                y[2 * i + 1] = s.y * p + s.x * q;
-            }
+                for (int i = 0; i < HALF / 2; ++i)
+                {
+                    const float2 r = cs[w + i];
+                    const float p = v[2 * i], q = v[2 * i + 1];
+                    v[2 * i] = r.x * p - r.y * q;
+                    v[2 * i + 1] = r.y * p + r.x * q;
+                }
+            };
+            turn(x, d0 / 2);
+            turn(y, d1 / 2);
         }
-        store4(row + d0, x);
-        store4(row + d1, y);
+        store_n<T, HALF>(row + d0, x);
+        store_n<T, HALF>(row + d1, y);
     }
 }
 
@@ -333,15 +402,20 @@ hipError_t launch_update_pages(hipStream_t st, const TView &cache, const TView &
     auto vec = [](const TView &t) {
         return t.s[3] == 1 && t.s[2] % 8 == 0 && t.s[1] % 8 == 0 && (uintptr_t)t.p % 16 == 0;
     };
-    const uint32_t T = k.n[1], all = cache.n[1] * (cache.n[3] / 8);
+    // 16 bytes of each half where heads allow it (a thread then moves 32); us for 4001 tokens of 32 key heads of 128 in fp16,
+    // pairs of halves: 8 bytes 31.2, 16 29.8 (28.0 on the GPU, 4.7 TB/s: a large copy's rate is 4.9)
+    const uint32_t hd = cache.n[3], half = cache.dt == DT_F16 && hd % 16 == 0 ? 8 : 4;
+    const uint32_t T = k.n[1], all = cache.n[1] * (hd / (2 * half));
     const uint32_t shares = min((all - 1) / 256 + 1, T >= 1024 ? 1u : (1023 / T) + 1);
     const uint32_t units = (all - 1) / shares + 1;
     const UpdatePagesArgs a{cache, k, v, map, map_s, units, vec(k) && vec(v), rope};
     const dim3 grid(T, shares);
-    if (cache.dt == DT_F16)
-        update_pages_kernel<_Float16><<<grid, 256, 0, st>>>(a);
+    if (cache.dt == DT_F32)
+        update_pages_kernel<float, 4><<<grid, 256, 0, st>>>(a);
+    else if (half == 8)
+        update_pages_kernel<_Float16, 8><<<grid, 256, 0, st>>>(a);
     else
-        update_pages_kernel<float><<<grid, 256, 0, st>>>(a);
+        update_pages_kernel<_Float16, 4><<<grid, 256, 0, st>>>(a);
     return hipGetLastError();
 }
 

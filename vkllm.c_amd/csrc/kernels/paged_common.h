@@ -7,6 +7,12 @@ namespace vk
 
 constexpr uint32_t kNoPage = 0xFFFFFFFFu;
 
+// 4 words at any word's address
+struct __attribute__((packed, aligned(4))) Word4
+{
+    u32x4 v;
+};
+
 // the workgroup meets; what it wrote to LDS is seen. Loads from memory stay in flight, which __syncthreads would wait for.
 __device__ __forceinline__ void lds_barrier()
 {

@@ -70,6 +70,28 @@ static vk::PagedRope rope_of(float base, bool neox, uint32_t hd)
     return r;
 }
 
+// The context's workspace and arrival counters, made at the first use and kept until the context is freed
+static vkllm_err_t paged_memory(vkllm_context *context, float **work, size_t *work_elems)
+{
+    vkllm_gpu_device *dev = context->device;
+    _CHECK(op_workspace(context, work, work_elems));
+    if (!*work)
+        return VKLLM_ERR_ALLOC;
+    if (dev->paged_arrivals)
+        return VKLLM_ERR_OK;
+    uint32_t *p = nullptr;
+    HIP_TRY(hipMalloc(&p, vk::kPagedArrivals * sizeof(uint32_t)));
+    hipError_t e = hipMemsetAsync(p, 0, vk::kPagedArrivals * sizeof(uint32_t), dev->stream);
+    if (e == hipSuccess)
+        e = hipStreamSynchronize(dev->stream);
+    if (e != hipSuccess)
+    {
+        (void)hipFree(p);
+        return hip_fail(e, "clearing the arrival counters", __FILE__, __LINE__);
+    }
+    dev->paged_arrivals = p;
+    return VKLLM_ERR_OK;
+}
 // =============================================================================================================
 // PAGE_TABLE
 extern "C" vkllm_err_t vkllm_op_page_table_init(struct vkllm_context *context, struct vkllm_commands *commands,
@@ -115,10 +137,13 @@ extern "C" vkllm_err_t vkllm_op_page_table_run(struct vkllm_context *context, st
         old = tview(context, tensor->srcs[1]);
         NEED_DEV(old);
     }
+    float *work = nullptr;
+    size_t work_elems = 0;
+    _CHECK(paged_memory(context, &work, &work_elems));
     LAUNCH(context, KID_PAGE_TABLE,
            vk::launch_page_table(context->device->stream, table_view(out), (const uint32_t *)old.p, old.s[2],
-                                 (const uint32_t *)want.p, want.s[3], p.page_rows, p.pages,
-                                 context->device->cu_count));
+                                 (const uint32_t *)want.p, want.s[3], p.page_rows, p.pages, work, work_elems,
+                                 context->device->paged_arrivals, context->device->cu_count));
     commands_note_write(commands, tensor);
     return VKLLM_ERR_OK;
 }
@@ -238,28 +263,6 @@ extern "C" vkllm_err_t vkllm_op_update_pages_post_run(struct vkllm_context *, st
 // =============================================================================================================
 // PAGED_ATTN
 
-// The context's workspace and arrival counters, made at the first use and kept until the context is freed
-static vkllm_err_t paged_attn_memory(vkllm_context *context, float **work, size_t *work_elems)
-{
-    vkllm_gpu_device *dev = context->device;
-    _CHECK(op_workspace(context, work, work_elems));
-    if (!*work)
-        return VKLLM_ERR_ALLOC;
-    if (dev->paged_arrivals)
-        return VKLLM_ERR_OK;
-    uint32_t *p = nullptr;
-    HIP_TRY(hipMalloc(&p, vk::kPagedArrivals * sizeof(uint32_t)));
-    hipError_t e = hipMemsetAsync(p, 0, vk::kPagedArrivals * sizeof(uint32_t), dev->stream);
-    if (e == hipSuccess)
-        e = hipStreamSynchronize(dev->stream);
-    if (e != hipSuccess)
-    {
-        (void)hipFree(p);
-        return hip_fail(e, "clearing the arrival counters", __FILE__, __LINE__);
-    }
-    dev->paged_arrivals = p;
-    return VKLLM_ERR_OK;
-}
 extern "C" vkllm_err_t vkllm_op_paged_attn_init(struct vkllm_context *context, struct vkllm_commands *commands,
                                                 struct vkllm_tensor *tensor)
 {
@@ -284,7 +287,7 @@ extern "C" vkllm_err_t vkllm_op_paged_attn_init(struct vkllm_context *context, s
     _CHECK_ARGS(std::isfinite(p.scale) && rope_base_ok(p.rope_base));
     float *work = nullptr;
     size_t work_elems = 0;
-    _CHECK(paged_attn_memory(context, &work, &work_elems));
+    _CHECK(paged_memory(context, &work, &work_elems));
     tensor->pipeline = pipeline_of(context, KID_PAGED_ATTN);
     return VKLLM_ERR_OK;
 }
@@ -307,7 +310,7 @@ extern "C" vkllm_err_t vkllm_op_paged_attn_run(struct vkllm_context *context, st
     NEED_DEV(out);
     float *work = nullptr;
     size_t work_elems = 0;
-    _CHECK(paged_attn_memory(context, &work, &work_elems));
+    _CHECK(paged_memory(context, &work, &work_elems));
     LAUNCH(context, KID_PAGED_ATTN,
            vk::launch_paged_attn(context->device->stream, q, cache, table_view(table), out, p.scale,
                                  rope_of(p.rope_base, p.neox_style, q.n[3]), work, work_elems,
@@ -341,6 +344,7 @@ extern "C" vkllm_err_t vkllm_op_adjust_logits_init(struct vkllm_context *context
     _CHECK_ARGS(x->strides[3] == dtype_bytes(x->dtype) && tensor->strides[3] == dtype_bytes(x->dtype));
     _CHECK_ARGS(!same_memory(tensor, x));
     const uint32_t B = x->shapes[2], V = x->shapes[3];
+    _CHECK_ARGS(B <= 65535); // a workgroup row each
     if (history)
         _CHECK_ARGS(rules && word_rows(history) && history->shapes[2] == B);
     if (rules)
