@@ -11,6 +11,8 @@
  * grows if its pages and those that the rows before it asked for are there; otherwise, and where the wanted length is
  * over P * page_rows, it stays as it was, which its first word tells. A length of 0 ends a sequence. Page ids at or past
  * `pages` in the table so far are carried along and occupy nothing.
+ * Captured into a hipGraph, the call is replayed on the context's stream, and has been run once before (otherwise it is
+ * refused).
  * The last page of a row that shares pages with another has to be full: tokens that follow go to pages of its own. */
 #ifndef VKLLM_OP_PAGE_TABLE_H
 #define VKLLM_OP_PAGE_TABLE_H

@@ -4,12 +4,14 @@
  * The tensor and srcs[0], the queries, are [1, B, H, head_dim] of any strides; srcs[1] is the cache (VKLLM_OP_UPDATE_PAGES,
  * [pages, 2 * KV, page_rows, head_dim], packed, page_rows a multiple of 16, H a multiple of KV: query head h reads key
  * head h / (H / KV)), all fp16 or all fp32; srcs[2] is the page table (VKLLM_OP_PAGE_TABLE, uint32 [1, 1, B, 1 + P], B <= 4096).
+ * P * page_rows is at most 2^31.
  * Row b is the last token of its sequence, whose keys and values the cache holds already: over positions j < length
  * out = sum_j softmax_j(scale * q . k_j) v_j, with q rotated to position length - 1 (unless rope_base is 0). Softmax and
- * sums are in 32 bits, and the result is rounded once. A row of length 0 gives zeros; lengths end at P * page_rows, and
- * positions on pages that the cache does not have count as absent. Rows of the cache past a sequence's end
- * are never used, whatever they hold.
- * _init sets up the context's workspace: code that captures _run into a hipGraph calls _init and _run once before. */
+ * sums are in 32 bits, and the result is rounded once. A row of length 0, and one whose every score is -inf, gives zeros;
+ * lengths end at P * page_rows, and positions on pages that the cache does not have count as absent. Rows of the cache
+ * past a sequence's end are never used, whatever they hold.
+ * Partial results go through a workspace of the context, made by _init: captured into a hipGraph, the call is replayed on
+ * the context's stream, and every tensor of it has been run once before (otherwise it is refused). */
 #ifndef VKLLM_OP_PAGED_ATTN_H
 #define VKLLM_OP_PAGED_ATTN_H
 #include <stdbool.h>

@@ -71,6 +71,20 @@ def test_adjust_logits(ctx, vk, B, V, T, N, dtype, pad):
 
 
 @pytest.mark.parametrize("dtype", [np.float16, np.float32])
+@pytest.mark.parametrize("V,T,N", [(40000, 70000, 5), (40000, 20, 33000), (100, 65534, 3), (100, 65535, 3)])
+def test_adjust_logits_past_16_bits(ctx, vk, V, T, N, dtype):
+    """Histories and biases longer than a half word counts: one token used more than 65535 times."""
+    print(f"[adjust_logits] V={V} T={T} N={N} {dtype.__name__}", flush=True)
+    r = np.random.default_rng(N)
+    x, history, rules, mask = make(r, 2, V, T, N, dtype)
+    history[0] = 7 % V
+    history[0, 0] = T
+    rules[:, 1] = np.float32(1e-4).view(np.uint32)
+    rules[:, 3] = N
+    check(run(ctx, vk, x, history, rules, mask), x, history, rules, mask)
+
+
+@pytest.mark.parametrize("dtype", [np.float16, np.float32])
 def test_adjust_logits_of_rows_that_nothing_is_left_of(ctx, vk, dtype):
     """All masked; NaN and infinities in masked places give -inf like any other; -inf logits stay; counts past a row end with it;
     rules that change nothing."""

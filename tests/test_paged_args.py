@@ -82,6 +82,15 @@ def slot_map(w, shape=(1, 1, 7, 2), table=(1, 1, 3, 9), lengths=(1, 1, 1, 3), co
                     V.SlotMapParams(rows))
 
 
+def test_slot_map_refuses_shared_memory(vk, world):
+    for i in range(3):
+        t = slot_map(world)
+        view = world.tensor(tuple(t.contents.srcs[i].contents.shapes), vk.U32, vk.OP_REF, [t])
+        view.contents.data.is_ref = True
+        t.contents.srcs[i] = view
+        assert world.init("slot_map", t) == vk.ERR_ARGS
+
+
 @pytest.mark.parametrize("kw", [
     dict(shape=(1, 1, 7, 3)), dict(shape=(1, 7, 1, 2)), dict(table=(1, 1, 4, 9)), dict(lengths=(1, 1, 1, 2)),
     dict(counts=(1, 1, 3, 1)), dict(rows=0), dict(dtype=1), dict(table=(1, 1, 3, 1))], ids=str)
@@ -133,7 +142,7 @@ def paged_attn(w, q=(1, 5, 6, 64), out=None, cache=(24, 6, 16, 64), table=(1, 1,
     dict(cache=(24, 6, 24, 64)), dict(cache=(24, 6, 8, 64)), dict(cache=(24, 3, 16, 64)), dict(table=(1, 1, 4, 9)),
     dict(table=(1, 1, 5, 1)), dict(q=(1, 5, 6, 60), cache=(24, 6, 16, 60)), dict(q=(1, 5, 6, 264), cache=(24, 6, 16, 264)),
     dict(scale=float("nan")), dict(scale=float("inf")), dict(base=-2.0), dict(dtype=4), dict(cd=1),
-    dict(q=(1, 4097, 6, 64), table=(1, 1, 4097, 9))], ids=str)
+    dict(q=(1, 4097, 6, 64), table=(1, 1, 4097, 9)), dict(cache=(2, 6, 65536, 64), table=(1, 1, 5, 32770))], ids=str)
 def test_paged_attn_refuses(vk, world, kw):
     # a description that passes goes on to the workspace, which needs a device: only refusals are asked for here
     assert world.init("paged_attn", paged_attn(world, **kw)) == vk.ERR_ARGS
@@ -159,7 +168,7 @@ def adjust(w, x=(1, 1, 3, 100), out=None, history=(1, 1, 3, 9), rules=(1, 1, 3, 
 @pytest.mark.parametrize("kw", [
     dict(out=(1, 1, 3, 99)), dict(x=(1, 3, 1, 100)), dict(history=(1, 1, 2, 9)), dict(rules=None), dict(rules=(1, 1, 3, 3)),
     dict(rules=(1, 1, 3, 7)), dict(rules=(1, 1, 4, 8)), dict(mask=(1, 1, 3, 3)), dict(mask=(1, 1, 1, 4)), dict(dtype=4),
-    dict(xd=1), dict(md=1)], ids=str)
+    dict(xd=1), dict(md=1), dict(x=(1, 1, 65536, 4), history=None, rules=None, mask=None)], ids=str)
 def test_adjust_logits_refuses(vk, world, kw):
     for ok in (dict(), dict(history=None), dict(history=None, rules=None), dict(mask=None), dict(dtype=vk.F32),
                dict(history=None, rules=None, mask=None), dict(mask=(1, 1, 3, 5))):

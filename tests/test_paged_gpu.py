@@ -276,6 +276,9 @@ ATTN = [  # lengths, H, KV, hd, R, base, neox, view
     ([20000], 4, 1, 128, 64, 1e4, True, None),              # split over many workgroups
     ([9000, 1, 0, 12345], 8, 8, 64, 16, 1e4, False, None),
     ([3] * 300 + [0] * 20 + [400] * 5, 4, 2, 64, 16, 1e4, False, None),  # more rows than threads
+    ([60000, 5], 16, 1, 64, 32, 1e4, False, None),          # joined over three levels, 16 heads a part
+    ([50000, 0, 30], 1, 1, 128, 16, 1e4, True, None),       # and with several threads to a pair of dims
+    ([700] * 65 + [0, 3000], 6, 3, 48, 16, 1e4, False, None),  # several rows to a workgroup, starts and ends counted
 ]
 
 
@@ -356,6 +359,34 @@ def test_paged_attn_of_infinities(ctx, vk):
     want, off = ref.attention(q[0], sane, table, 0.125, 0.0, False)
     for b, h in ((0, 1), (1, 0), (2, 1), (3, 0), (3, 1)):
         assert (np.abs(got[b, h] - want[b, h]) <= half_step(want[b, h], np.float16) * 1.001 + off[b, h]).all()
+
+
+@pytest.mark.parametrize("dtype", [np.float16, np.float32])
+def test_paged_attn_of_an_undefined_query(ctx, vk, dtype):
+    """A query that is not a number makes its head undefined, also where parts of the row are joined, and no other."""
+    r = np.random.default_rng(6)
+    q, cache, table = make_attention(r, [12000, 90], 4, 2, 64, 16, dtype)
+    q[0, :, 2, 5] = np.nan
+    got = run_attention(ctx, vk, q, cache, table, 0.125, 1e4, False)
+    assert np.isnan(got[:, 2]).all()
+    q[0, :, 2, 5] = 0
+    want, off = ref.attention(q[0], cache, table, 0.125, 1e4, False)
+    for h in (0, 1, 3):
+        assert (np.abs(got[:, h] - want[:, h]) <= half_step(want[:, h], dtype) * 1.001 + off[:, h]).all()
+
+
+def test_paged_attn_into_a_permuted_tensor(ctx, vk):
+    """The result's own order of memory is another one: [H, B, hd] seen as [B, H, hd]."""
+    r = np.random.default_rng(12)
+    q, cache, table = make_attention(r, [40, 0, 300], 6, 2, 64, 16, np.float16)
+    with Bag(ctx) as bag:
+        t = ctx.tensor([1, 6, 3, 64], vk.F16, op=vk.OP_PAGED_ATTN, srcs=[bag.put(q), bag.put(cache), bag.put(rows4(table))],
+                       params=vk.PagedAttnParams(0.125, 1e4, False))
+        bag.made.append(t)
+        vk.check("permute", vk.lib().vkllm_tensor_permute(ctx.vp, t, (ctypes.c_uint32 * 4)(0, 2, 1, 3)))
+        vk.check("paged_attn", ctx.run_op("paged_attn", t))
+        got = ctx.download(t)[0]
+    check_attention(got, q, cache, table, 0.125, 1e4, False)
 
 
 def test_paged_attn_past_32_bit_offsets(ctx, vk):

@@ -8,7 +8,7 @@ import ctypes
 import numpy as np
 import pytest
 
-from paged_ref import rotate
+from paged_ref import attention, rotate
 from test_paged_gpu import Bag, rows4
 from test_zz_no_alloc import _hip_runtime
 
@@ -236,3 +236,31 @@ def test_a_captured_step_replays(ctx, vk, tiny):
                 H.hipGraphExecDestroy(exe)
             if graph.value:
                 H.hipGraphDestroy(graph)
+
+
+def test_a_first_call_under_capture_is_refused(ctx, vk):
+    """An operator whose result has no memory yet cannot make it while the stream is captured: it says so, the capture goes on,
+    and the same call works afterwards."""
+    H, L = _hip_runtime(), vk.lib()
+    stream, graph = ctypes.c_void_p(), ctypes.c_void_p()
+    vk.check("stream", L.vkllm_hip_context_stream(ctx.vp, ctypes.byref(stream)))
+    r = np.random.default_rng(1)
+    q, cache = (r.standard_normal(s).astype(np.float16) for s in ((1, 2, 4, 64), (5, 4, 16, 64)))
+    table = np.array([[20, 0, 1], [3, 4, 0xFFFFFFFF]], np.uint32)
+    with Bag(ctx) as bag:
+        t = ctx.tensor([1, 2, 4, 64], vk.F16, op=vk.OP_PAGED_ATTN, srcs=[bag.put(q), bag.put(cache), bag.put(rows4(table))],
+                       params=vk.PagedAttnParams(0.125, 0.0, False))
+        x = bag.put(r.standard_normal((1, 1, 2, 100)).astype(np.float16))
+        y = ctx.tensor([1, 1, 2, 100], vk.F16, op=vk.OP_ADJUST_LOGITS, srcs=[x])
+        bag.made += [t, y]
+        assert H.hipStreamBeginCapture(stream, 0) == 0
+        rcs = [L.vkllm_op_paged_attn_run(ctx.vp, ctx.cmds, t), L.vkllm_op_adjust_logits_run(ctx.vp, ctx.cmds, y)]
+        assert H.hipStreamEndCapture(stream, ctypes.byref(graph)) == 0
+        if graph.value:
+            H.hipGraphDestroy(graph)
+        assert rcs == [vk.ERR_ARGS, vk.ERR_ARGS]
+        vk.check("paged_attn", ctx.run_op("paged_attn", t))
+        vk.check("adjust_logits", ctx.run_op("adjust_logits", y))
+        want, off = attention(q[0], cache, table, 0.125, 0.0, False)
+        assert (np.abs(ctx.download(t)[0] - want) <= np.abs(want) * 2.0 ** -11 * 1.001 + off + 2.0 ** -25).all()
+        assert np.array_equal(ctx.download(y), ctx.download(x))

@@ -77,22 +77,31 @@ template <typename T, bool WIDE> __global__ __launch_bounds__(1024) void adjust_
     uint32_t my_bias = ~0u;
     if (rules)
     {
-        n_bias = min(rules[3], (a.rules.n - 4) / 2);
-        rep = __uint_as_float(rules[0]);
-        inverse = 1.f / rep; // a product instead of a division per token: off by one roundoff of 32 bits more
-        freq = __uint_as_float(rules[1]);
-        pres = __uint_as_float(rules[2]);
+        // everything is asked for as far as its row goes, and cut to what the row has of it when that is known
+        const uint32_t most_biases = (a.rules.n - 4) / 2;
+        if (t < most_biases)
+            my_bias = rules[4 + 2 * t];
+        float value = t < most_biases ? __uint_as_float(rules[5 + 2 * t]) : 0.f;
         if (a.history.p)
         {
             h = a.history.p + (size_t)b * a.history.stride + 1;
-            used = min(h[-1], a.history.n - 1);
-            if (t < used / 4)
+            if (t < (a.history.n - 1) / 4)
                 mine = ((const Word4 *)h)[t].v;
+            used = min(scalar_word(h - 1), a.history.n - 1);
         }
-        if (t < n_bias)
-            my_bias = rules[4 + 2 * t];
+        n_bias = min(scalar_word(rules + 3), most_biases);
+        rep = __uint_as_float(scalar_word(rules));
+        inverse = 1.f / rep; // a product instead of a division per token: off by one roundoff of 32 bits more
+        freq = __uint_as_float(scalar_word(rules + 1));
+        pres = __uint_as_float(scalar_word(rules + 2));
+        if (t >= used / 4)
+            mine = (u32x4){~0u, ~0u, ~0u, ~0u};
         for (uint32_t i = t; i < min(n_bias, kBiasesInLds); i += threads)
-            values[i] = __uint_as_float(rules[5 + 2 * i]);
+        {
+            values[i] = value;
+            if (i + threads < min(n_bias, kBiasesInLds))
+                value = __uint_as_float(rules[5 + 2 * (i + threads)]);
+        }
         for (uint32_t i = t; i < (WIDE ? 2 : 1) * tile / 4; i += threads)
             ((u32x4 *)lds)[i] = (u32x4){0, 0, 0, 0};
     }

@@ -8,8 +8,8 @@
 // Work is split without knowing the lengths on the host: a unit is KT consecutive positions of one (sequence, key head),
 // all units of the batch are numbered in that order, and each of a fixed number of workgroups (as many as are resident)
 // takes an equal run of them. A (sequence, head) that ends up in several workgroups leaves partial sums in the workspace,
-// and whichever workgroup of a group of them is the last to arrive joins the group's, up a tree (join_up below). A workgroup
-// finds its units from prefix sums of the lengths, formed in LDS.
+// and whichever workgroup of a group of them is the last to arrive joins the group's, up a tree. A workgroup finds
+// its units from prefix sums of the lengths, formed in LDS.
 //
 // Matrix cores do the products although 16 - G of their 16 columns are idle when G heads share a key head: they have 24
 // times the rate that the cache arrives at, and the layout spares the shuffles that dot products of single rows need.
@@ -53,9 +53,9 @@ struct PagedAttnArgs
 };
 
 // a partial result: o [tile_heads][hd], then (m, l) [tile_heads]
-__host__ __device__ __forceinline__ size_t part_floats(uint32_t tile_heads, uint32_t hd)
+__host__ __device__ __forceinline__ uint32_t part_floats(uint32_t tile_heads, uint32_t hd)
 {
-    return (size_t)tile_heads * (hd + 2);
+    return tile_heads * (hd + 2);
 }
 
 // Two floats of a partial result, written through to the level that all XCDs share and read from there: no workgroup needs
@@ -96,6 +96,12 @@ template <bool F16, int HDP> struct PagedTile
     static constexpr int PER_CU = HDP == 256 ? 1 : 2;
 };
 
+// n / d, d > 0, by the much shorter 32-bit division where that is the same
+__device__ __forceinline__ uint64_t quotient(uint64_t n, uint64_t d)
+{
+    return (n | d) >> 32 ? n / d : (uint32_t)n / (uint32_t)d;
+}
+
 __device__ __forceinline__ float exp2_of(float x)
 {
     return __builtin_amdgcn_exp2f(x);
@@ -104,7 +110,7 @@ __device__ __forceinline__ float exp2_of(float x)
 // dynamic LDS: lengths [B], queries [QN][16][QP], per-wave statistics [4][16][2], per-wave sums [4][tile_heads][hd]
 // FULL: head_dim is HDP, else it is smaller
 template <bool F16, int HDP, bool FULL>
-__global__ __launch_bounds__(256, HDP == 256 ? 1 : HDP == 64 ? 4 : 2) void paged_attn_kernel(PagedAttnArgs a)
+__global__ __launch_bounds__(256, HDP == 256 ? 1 : 2) void paged_attn_kernel(PagedAttnArgs a)
 {
     using Tile = PagedTile<F16, HDP>;
     using T = typename std::conditional<F16, _Float16, float>::type;
@@ -118,7 +124,7 @@ __global__ __launch_bounds__(256, HDP == 256 ? 1 : HDP == 64 ? 4 : 2) void paged
     // the rows whose parts lie in slots 0 and 1: how many parts they have, and the number of this one
     struct Split
     {
-        uint32_t b, hg, parts, number;
+        uint32_t b, head0, heads, parts, number;
     };
     __shared__ Split split[2];
     const uint32_t t = threadIdx.x, lane = t % kWave, wave = __builtin_amdgcn_readfirstlane(t / kWave);
@@ -127,14 +133,6 @@ __global__ __launch_bounds__(256, HDP == 256 ? 1 : HDP == 64 ? 4 : 2) void paged
     uint32_t *lens = lds;
     T *qs = (T *)(lens + (B + 3) / 4 * 4);
     float *ml = (float *)(qs + QN * kHeadsPerTile * QP), *sums = ml + 4 * kHeadsPerTile * 2;
-
-    // rows of the queries that stay zero, and dims past the head
-    for (uint32_t i = t; i < QN * kHeadsPerTile * (QP / 4); i += 256)
-        if (i / (QP / 4) % kHeadsPerTile >= a.tile_heads || i % (QP / 4) * 4 >= hd)
-            for (uint32_t k = 0; k < 4; ++k)
-                qs[4 * i + k] = (T)0.f;
-    if (t < 2)
-        split[t].parts = 0;
 
     // Units of every row, and this workgroup's run of them. A (sequence, head) counts `extra` units more, before its first:
     // what starting and ending it costs. A sum holds units in its low 40 bits and rows that have any above.
@@ -145,23 +143,31 @@ __global__ __launch_bounds__(256, HDP == 256 ? 1 : HDP == 64 ? 4 : 2) void paged
     };
     auto units_of = [&](uint32_t len) { return (uint32_t)((len + (uint64_t)KT - 1) / KT); };
     auto count_of = [&](uint32_t len) { return units_of(len) | (uint64_t)(len > 0) << 40; };
+    const uint32_t len0 = lane < B ? len_of(lane) : 0; // asked for before anything else
+    // rows of the queries that stay zero, and dims past the head
+    for (uint32_t i = t; i < QN * kHeadsPerTile * (QP / 4); i += 256)
+        if (i / (QP / 4) % kHeadsPerTile >= a.tile_heads || i % (QP / 4) * 4 >= hd)
+            for (uint32_t k = 0; k < 4; ++k)
+                qs[4 * i + k] = (T)0.f;
+    if (t < 2)
+        split[t].parts = 0;
+
     uint32_t extra;
     uint64_t share, u0, u1, base; // base: the number of the first row's first unit
     uint32_t row0;                // the first row
     auto weigh = [&](uint64_t sum) { return ((sum & ((1ull << 40) - 1)) + extra * (sum >> 40)) * heads; };
     auto divide = [&](uint64_t total) {
         extra = (total & ((1ull << 40) - 1)) * heads > 4 * gridDim.x ? kSegmentUnits : 0;
-        share = (weigh(total) + gridDim.x - 1) / gridDim.x;
+        share = quotient(weigh(total) + gridDim.x - 1, gridDim.x);
         u0 = blockIdx.x * share;
         u1 = min(u0 + share, weigh(total));
     };
     if (B <= kWave)
     {
         // every wave for itself
-        const uint32_t len = lane < B ? len_of(lane) : 0;
         if (lane < B)
-            lens[lane] = len;
-        const uint64_t mine = count_of(len), upto = wave_scan(mine);
+            lens[lane] = len0;
+        const uint64_t mine = count_of(len0), upto = wave_scan(mine);
         divide(read_lane(upto, kWave - 1));
         const uint64_t found = __ballot(u0 < weigh(upto) && u0 >= weigh(upto - mine));
         row0 = found ? __ffsll((unsigned long long)found) - 1 : 0;
@@ -198,11 +204,11 @@ __global__ __launch_bounds__(256, HDP == 256 ? 1 : HDP == 64 ? 4 : 2) void paged
     if (u0 >= u1)
         return;
 
-    // A unit's place: sequence b of `len` positions and n units per head, tile hg of its query heads, unit s of number v. The
-    // same for the whole workgroup, so it is kept in scalar registers.
+    // A unit's place: sequence b of `len` positions and n units per head, key head h and tile g of its query heads, unit s of
+    // number v. The same for the whole workgroup, so it is kept in scalar registers.
     struct Place
     {
-        uint32_t b, len, n, hg, s;
+        uint32_t b, len, n, h, g, s;
         uint32_t v; // behind u0
     };
     auto row_at = [&](Place &p, uint32_t b) {
@@ -218,10 +224,14 @@ __global__ __launch_bounds__(256, HDP == 256 ? 1 : HDP == 64 ? 4 : 2) void paged
         {
             p.s = 0;
             p.v += extra;
-            if (++p.hg == heads)
+            if (++p.g == a.groups)
             {
-                p.hg = 0;
-                row_at(p, min(p.b + 1, B - 1));
+                p.g = 0;
+                if (++p.h == a.KV)
+                {
+                    p.h = 0;
+                    row_at(p, min(p.b + 1, B - 1));
+                }
             }
         }
         return p;
@@ -229,9 +239,10 @@ __global__ __launch_bounds__(256, HDP == 256 ? 1 : HDP == 64 ? 4 : 2) void paged
     Place cur;
     row_at(cur, __builtin_amdgcn_readfirstlane(row0));
     {
-        const uint64_t rel = u0 - base, n = cur.n + extra;
-        const uint32_t at = (uint32_t)(rel % n);
-        cur.hg = __builtin_amdgcn_readfirstlane((uint32_t)(rel / n));
+        const uint64_t rel = u0 - base;
+        const uint32_t n = cur.n + extra, hg = (uint32_t)quotient(rel, n), at = (uint32_t)(rel - (uint64_t)hg * n);
+        cur.h = __builtin_amdgcn_readfirstlane(hg / a.groups);
+        cur.g = __builtin_amdgcn_readfirstlane(hg % a.groups);
         cur.s = __builtin_amdgcn_readfirstlane(at < extra ? 0 : at - extra);
         cur.v = __builtin_amdgcn_readfirstlane(at < extra ? extra - at : 0);
     }
@@ -239,9 +250,9 @@ __global__ __launch_bounds__(256, HDP == 256 ? 1 : HDP == 64 ? 4 : 2) void paged
     if (cur.v >= end)
         return;
 
-    auto head_of = [&](const Place &p) { return p.hg / a.groups; };
-    auto head0_of = [&](const Place &p) { return head_of(p) * a.G + p.hg % a.groups * kHeadsPerTile; };
-    auto heads_of = [&](const Place &p) { return min((uint32_t)kHeadsPerTile, (head_of(p) + 1) * a.G - head0_of(p)); };
+    // its query heads: the first of them, and how many
+    auto head0_of = [&](const Place &p) { return p.h * a.G + p.g * kHeadsPerTile; };
+    auto heads_of = [&](const Place &p) -> uint32_t { return min((uint32_t)kHeadsPerTile, a.G - p.g * kHeadsPerTile); };
 
     // Queries and their pairs' frequencies: thread t has pairs t + 256 j of tile_heads heads (the other rows in LDS stay
     // zero). They are asked for before the keys of their first unit, and staged when the unit before is done with.
@@ -319,7 +330,7 @@ __global__ __launch_bounds__(256, HDP == 256 ? 1 : HDP == 64 ? 4 : 2) void paged
             const bool there = tile <= (p.len - 1) / 16 && pid[i] < a.pages;
             live[i] = there ? min(16u, p.len - tile * 16) : 0u;
             const uint32_t in_page = tile - page_of(tile) * a.page_tiles;
-            const size_t at = (size_t)pid[i] * a.page_bytes + (head_of(p) * a.head_bytes + in_page * (16 * hd * ES));
+            const size_t at = (size_t)pid[i] * a.page_bytes + (p.h * a.head_bytes + in_page * (16 * hd * ES));
             rows[i] = (const char *)a.cache + (there ? at : 0);
         }
     };
@@ -519,7 +530,7 @@ __global__ __launch_bounds__(256, HDP == 256 ? 1 : HDP == 64 ? 4 : 2) void paged
         to[0] = (T)(lsum == 0.f ? 0.f : o0 / lsum); // a row of no weight is zero
         to[a.os[2]] = (T)(lsum == 0.f ? 0.f : o1 / lsum);
     };
-    // What the workgroup has of (sequence, heads) p.b, p.hg: its units from `from` to p.s
+    // What the workgroup has of p's sequence and heads: its units from `from` to p.s
     auto finish = [&](const Place &p, uint32_t from) {
         const uint32_t Gn = heads_of(p), head0 = head0_of(p);
         l += __shfl_xor(l, 16, kWave);
@@ -542,10 +553,12 @@ __global__ __launch_bounds__(256, HDP == 256 ? 1 : HDP == 64 ? 4 : 2) void paged
         lds_barrier();
         const bool all = from == 0 && p.s + 1 == p.n;
         // a row that began in another workgroup leaves its part in slot 0, one that goes on in the next in slot 1
-        float *part = a.parts + (2 * (size_t)blockIdx.x + (from == 0 ? 1 : 0)) * part_floats(a.tile_heads, hd);
-        for (uint32_t e = 2 * t; e < Gn * hd; e += 512)
+        float *part = a.parts + (2 * blockIdx.x + (from == 0 ? 1 : 0)) * part_floats(a.tile_heads, hd);
+        for (uint32_t e = t; e < Gn * (HDP / 2); e += 256)
         {
-            const uint32_t i = e / hd, d = e % hd;
+            const uint32_t i = e / (HDP / 2), d = e % (HDP / 2) * 2;
+            if (!FULL && d >= hd)
+                continue;
             float mw[4], top = kNegInf, lsum = 0.f, o0 = 0.f, o1 = 0.f;
 #pragma unroll
             for (int w = 0; w < 4; ++w)
@@ -566,7 +579,7 @@ __global__ __launch_bounds__(256, HDP == 256 ? 1 : HDP == 64 ? 4 : 2) void paged
                 store_out(p.b, head0 + i, d, o0, o1, lsum);
             else
             {
-                put2(part + e, o0, o1);
+                put2(part + i * hd + d, o0, o1);
                 if (d == 0)
                     put2(part + a.tile_heads * hd + 2 * i, top, lsum);
             }
@@ -586,9 +599,10 @@ __global__ __launch_bounds__(256, HDP == 256 ? 1 : HDP == 64 ? 4 : 2) void paged
     lds_barrier();
     uint32_t from = cur.s;
     auto note = [&](const Place &p, uint32_t from) {
-        const uint32_t before = (uint32_t)((from + share - 1) / share), behind = (uint32_t)((p.n - p.s - 1 + share - 1) / share);
+        const uint32_t before = (uint32_t)quotient(from + share - 1, share),
+                       behind = (uint32_t)quotient(p.n - p.s - 1 + share - 1, share);
         if (t == 0)
-            split[from == 0] = {p.b, p.hg, before + 1 + behind, before};
+            split[from == 0] = {p.b, head0_of(p), heads_of(p), before + 1 + behind, before};
     };
     while (next.v < end)
     {
@@ -622,14 +636,14 @@ __global__ __launch_bounds__(256, HDP == 256 ? 1 : HDP == 64 ? 4 : 2) void paged
         uint32_t n = __builtin_amdgcn_readfirstlane(split[which].parts);
         if (n == 0)
             continue;
-        const uint32_t hg = __builtin_amdgcn_readfirstlane(split[which].hg), head0 = hg / a.groups * a.G + hg % a.groups * kHeadsPerTile;
-        const uint32_t Gn = min((uint32_t)kHeadsPerTile, (hg / a.groups + 1) * a.G - head0);
+        const uint32_t head0 = __builtin_amdgcn_readfirstlane(split[which].head0),
+                       Gn = __builtin_amdgcn_readfirstlane(split[which].heads);
         uint32_t k = __builtin_amdgcn_readfirstlane(split[which].number), stride = 1;
-        const uint32_t first = blockIdx.x - k, pairs = Gn * hd / 2;
+        const uint32_t first = blockIdx.x - k, pairs = Gn * (HDP / 2);
         const uint32_t ways = join_ways(pairs), fan = kJoinFan * ways;
-        const size_t floats = part_floats(a.tile_heads, hd), half = 2 * gridDim.x * floats;
+        const uint32_t floats = part_floats(a.tile_heads, hd), half = 2 * gridDim.x * floats; // of 2^26 at most
         // the place of part k: the first part's row starts in its workgroup, the others' does not
-        auto slot = [&](uint32_t k) { return 2 * (size_t)(first + k) + (k == 0 ? 1 : 0); };
+        auto slot = [&](uint32_t k) { return 2 * (first + k) + (k == 0 ? 1 : 0); };
         for (uint32_t level = 0;; ++level)
         {
             const uint32_t group = k / fan, size = min(fan, n - group * fan), lead = group * fan * stride;
@@ -637,7 +651,7 @@ __global__ __launch_bounds__(256, HDP == 256 ? 1 : HDP == 64 ? 4 : 2) void paged
             __syncthreads();
             if (t == 0)
             {
-                uint32_t *counter = a.arrivals + 2 * (size_t)level * gridDim.x + slot(lead);
+                uint32_t *counter = a.arrivals + 2 * level * gridDim.x + slot(lead);
                 arrived = __hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
                 if (arrived == size - 1)
                     __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); // for the next launch
@@ -648,15 +662,16 @@ __global__ __launch_bounds__(256, HDP == 256 ? 1 : HDP == 64 ? 4 : 2) void paged
             // levels write one half of the workspace and read the other, so nothing is overwritten that is still read
             const float *in = a.parts + (level % 2) * half;
             float *to = a.parts + (1 - level % 2) * half + slot(lead) * floats;
-            // (m, l, o, o) of pair e from parts way, way + ways, ... of the group
+            // (m, l, o, o) of pair e from parts way, way + ways, ... of the group (dims past the head repeat its last)
             auto gather = [&](uint32_t e, uint32_t way) {
                 float2 o[kJoinFan], ml[kJoinFan];
+                const uint32_t i = e / (HDP / 2), d = min(e % (HDP / 2) * 2, hd - 2);
 #pragma unroll
                 for (uint32_t c = 0; c < kJoinFan; ++c)
                 {
                     const float *part = in + slot(lead + min(way + c * ways, size - 1) * stride) * floats;
-                    o[c] = get2(part + 2 * e);
-                    ml[c] = get2(part + a.tile_heads * hd + 2 * (2 * e / hd));
+                    o[c] = get2(part + i * hd + d);
+                    ml[c] = get2(part + a.tile_heads * hd + 2 * i);
                 }
                 float m = kNegInf;
 #pragma unroll
@@ -669,22 +684,24 @@ __global__ __launch_bounds__(256, HDP == 256 ? 1 : HDP == 64 ? 4 : 2) void paged
                 f32x4 r = {m, 0.f, 0.f, 0.f};
 #pragma unroll
                 for (uint32_t c = 0; c < kJoinFan; ++c)
-                    if (ml[c].x != kNegInf)
-                    {
-                        const float f = exp2_of(ml[c].x - m);
-                        r[1] += f * ml[c].y;
-                        r[2] += f * o[c].x;
-                        r[3] += f * o[c].y;
-                    }
+                {
+                    // a part without a largest score counts with 0, which keeps a sum that is not a number one
+                    const float f = ml[c].x == kNegInf ? 0.f : exp2_of(ml[c].x - m);
+                    r[1] += f * ml[c].y;
+                    r[2] += f * o[c].x;
+                    r[3] += f * o[c].y;
+                }
                 return r;
             };
             auto emit = [&](uint32_t e, f32x4 r) {
-                const uint32_t i = 2 * e / hd, d = 2 * e % hd;
+                const uint32_t i = e / (HDP / 2), d = e % (HDP / 2) * 2;
+                if (!FULL && d >= hd)
+                    return;
                 if (n <= fan)
                     store_out(split[which].b, head0 + i, d, r[2], r[3], r[1]);
                 else
                 {
-                    put2(to + 2 * e, r[2], r[3]);
+                    put2(to + i * hd + d, r[2], r[3]);
                     if (d == 0)
                         put2(to + a.tile_heads * hd + 2 * i, r[0], r[1]);
                 }
@@ -706,13 +723,10 @@ __global__ __launch_bounds__(256, HDP == 256 ? 1 : HDP == 64 ? 4 : 2) void paged
                     for (uint32_t w = 0; w < ways; ++w)
                     {
                         const f32x4 x = joined[w * pairs + t];
-                        if (x[0] != kNegInf)
-                        {
-                            const float f = exp2_of(x[0] - m);
-                            r[1] += f * x[1];
-                            r[2] += f * x[2];
-                            r[3] += f * x[3];
-                        }
+                        const float f = x[0] == kNegInf ? 0.f : exp2_of(x[0] - m);
+                        r[1] += f * x[1];
+                        r[2] += f * x[2];
+                        r[3] += f * x[3];
                     }
                     emit(t, r);
                 }

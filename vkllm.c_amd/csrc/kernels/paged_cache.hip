@@ -20,7 +20,7 @@ namespace vk
 // which hang on a row's own lengths only: the kept ids (unless in place) and NO_PAGE behind. One launch. Bound by latency
 // and by a CU's rate of LDS atomics: 256 rows of up to 512 pages of 65536 take 11.8 us, 16.8 with one marking workgroup;
 // 1000 rows of up to 700 of 400000 with slots and positions of 8000 tokens 33 us, 58 with five.
-constexpr int kTableThreads = 1024;
+constexpr uint32_t kMaxTableThreads = 1024, kMinTableThreads = 256;
 
 struct PageTableArgs
 {
@@ -54,10 +54,10 @@ __device__ __forceinline__ RowPages row_pages(uint32_t had, uint32_t want, uint3
     return {had, want, keep, ceil_pages(want, R) - keep};
 }
 
-__global__ __launch_bounds__(kTableThreads) void page_table_kernel(PageTableArgs a)
+__global__ __launch_bounds__(kMaxTableThreads) void page_table_kernel(PageTableArgs a)
 {
     extern __shared__ uint32_t lds[];
-    const uint32_t t = threadIdx.x, B = a.out.B, P = a.out.P, R = a.R;
+    const uint32_t t = threadIdx.x, threads = blockDim.x, B = a.out.B, P = a.out.P, R = a.R;
     if (blockIdx.x >= a.markers)
     {
         // the columns of rows b, b + (such workgroups), ...: a thread per column
@@ -67,13 +67,13 @@ __global__ __launch_bounds__(kTableThreads) void page_table_kernel(PageTableArgs
             uint32_t *to = a.out.p + (size_t)b * a.out.stride + 1;
             if (!a.old)
             {
-                for (uint32_t c = (want > (uint64_t)P * R ? P : ceil_pages(want, R)) + t; c < P; c += kTableThreads)
+                for (uint32_t c = (want > (uint64_t)P * R ? P : ceil_pages(want, R)) + t; c < P; c += threads)
                     to[c] = kNoPage;
                 continue;
             }
             const uint32_t *from = a.old + (size_t)b * a.old_stride;
             const RowPages r = row_pages(from[0], want, R, P);
-            for (uint32_t c = t; c < P; c += kTableThreads)
+            for (uint32_t c = t; c < P; c += threads)
                 if (c < r.keep || c >= r.keep + r.need)
                     to[c] = c < r.keep ? from[1 + c] : kNoPage;
         }
@@ -82,14 +82,14 @@ __global__ __launch_bounds__(kTableThreads) void page_table_kernel(PageTableArgs
     const uint32_t words = (a.pages + 63) / 64 * 2;
     uint32_t *used = lds, *start = used + words, *keeps = start + B + 1, *hads = keeps + B, *wants = hads + B,
              *ranks = wants + B;
-    __shared__ uint64_t scan[kTableThreads / kWave];
+    __shared__ uint64_t scan[kMaxTableThreads / kWave];
     __shared__ uint32_t arrived;
     const uint32_t *old = a.old ? a.old : a.out.p;
     const uint32_t old_stride = a.old ? a.old_stride : a.out.stride;
-    for (uint32_t w = t; w < words; w += kTableThreads) // bits past the last page count as used
+    for (uint32_t w = t; w < words; w += threads) // bits past the last page count as used
         used[w] = w * 32 + 32 <= a.pages ? 0u : w * 32 >= a.pages ? ~0u : ~0u << (a.pages % 32);
     // demands, summed in row order: thread t has rows t * per .. t * per + per - 1
-    const uint32_t per = (B + kTableThreads - 1) / kTableThreads;
+    const uint32_t per = (B + threads - 1) / threads;
     uint64_t mine = 0;
     for (uint32_t b = t * per; b < t * per + per && b < B; ++b)
     {
@@ -112,7 +112,7 @@ __global__ __launch_bounds__(kTableThreads) void page_table_kernel(PageTableArgs
         start[B] = (uint32_t)total;
     __syncthreads();
     // Marks: a wave takes 256 columns of 4 rows at a time, neighbouring lanes neighbouring columns, 16 ids a lane on their way
-    const uint32_t lane = t % kWave, wave = __builtin_amdgcn_readfirstlane(t / kWave), waves = kTableThreads / kWave;
+    const uint32_t lane = t % kWave, wave = __builtin_amdgcn_readfirstlane(t / kWave), waves = threads / kWave;
     const uint32_t chunks = (P - 1) / kMarkColumns + 1, rows = (B - 1) / a.markers + 1, first = blockIdx.x * rows;
     const uint32_t items = first < B ? min(rows, B - first) * chunks : 0;
     for (uint32_t i0 = wave * 4; i0 < items; i0 += waves * 4)
@@ -146,7 +146,7 @@ __global__ __launch_bounds__(kTableThreads) void page_table_kernel(PageTableArgs
     {
         uint64_t *bits = (uint64_t *)a.bits;
         const uint64_t *mine = (const uint64_t *)used;
-        for (uint32_t w = t; w < words / 2; w += kTableThreads)
+        for (uint32_t w = t; w < words / 2; w += threads)
             __hip_atomic_store(bits + (size_t)blockIdx.x * (words / 2) + w, mine[w], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         __builtin_amdgcn_s_waitcnt(0); // this thread's bits are there
         __syncthreads();
@@ -159,7 +159,7 @@ __global__ __launch_bounds__(kTableThreads) void page_table_kernel(PageTableArgs
         __syncthreads();
         if (arrived != a.markers - 1)
             return;
-        for (uint32_t w = t; w < words / 2; w += kTableThreads)
+        for (uint32_t w = t; w < words / 2; w += threads)
         {
             uint64_t any = mine[w];
 #pragma unroll 8
@@ -170,7 +170,7 @@ __global__ __launch_bounds__(kTableThreads) void page_table_kernel(PageTableArgs
         __syncthreads();
     }
     // free pages before thread t's words
-    const uint32_t wper = (words + kTableThreads - 1) / kTableThreads;
+    const uint32_t wper = (words + threads - 1) / threads;
     uint64_t free_mine = 0;
     for (uint32_t w = t * wper; w < t * wper + wper && w < words; ++w)
         free_mine += __popc(~used[w]);
@@ -181,9 +181,9 @@ __global__ __launch_bounds__(kTableThreads) void page_table_kernel(PageTableArgs
     // The k-th free page to the row with start[b] <= k < start[b + 1], a thread per k: the page is found from the ranks of the
     // threads' words, counts of bits and halves of a word
     const uint32_t last = (uint32_t)(total < nfree ? total : nfree);
-    for (uint32_t k = t; k < last; k += kTableThreads)
+    for (uint32_t k = t; k < last; k += threads)
     {
-        const uint32_t owner = last_at_most(ranks, kTableThreads, k);
+        const uint32_t owner = last_at_most(ranks, threads, k);
         uint32_t w = owner * wper, nth = k - ranks[owner], at = 0;
         for (; nth >= (uint32_t)__popc(~used[w]); ++w)
             nth -= __popc(~used[w]);
@@ -203,7 +203,7 @@ __global__ __launch_bounds__(kTableThreads) void page_table_kernel(PageTableArgs
             a.out.p[(size_t)b * a.out.stride + 1 + keeps[b] + (k - start[b])] = w * 32 + at;
     }
     // lengths, and NO_PAGE where a row that does not fit would have had its pages
-    for (uint32_t b = t; b < B; b += kTableThreads)
+    for (uint32_t b = t; b < B; b += threads)
     {
         const uint32_t need = start[b + 1] - start[b];
         const bool fits = need == 0 || (uint64_t)start[b] + need <= nfree;
@@ -220,7 +220,7 @@ hipError_t launch_page_table(hipStream_t st, const PageTableView &out, const uin
                              size_t work_elems, uint32_t *arrivals, int cu_count)
 {
     const uint32_t words = (pages + 63) / 64 * 2;
-    const size_t lds = (words + 4 * (size_t)out.B + 1 + kTableThreads) * 4; // 132 KB at most
+    const size_t lds = (words + 4 * (size_t)out.B + 1 + kMaxTableThreads) * 4; // 132 KB at most
     static uint64_t done = 0;
     const hipError_t e = lds_attr_once((const void *)page_table_kernel, 134 << 10, done);
     if (e != hipSuccess)
@@ -230,7 +230,10 @@ hipError_t launch_page_table(hipStream_t st, const PageTableView &out, const uin
     const uint32_t markers = (uint32_t)std::max<uint64_t>(
         1, std::min<uint64_t>({out.B, pieces / kMarkPieces, kMaxMarkers, (256 << 10) / words, work_elems / words}));
     const uint32_t fill = std::min(out.B, (uint32_t)cu_count);
-    page_table_kernel<<<markers + fill, kTableThreads, lds, st>>>(PageTableArgs{
+    // a small table takes fewer waves to bring together: a row of up to 256 pages of 256 takes 4.7 us with 1024 threads,
+    // 3.4 with 256; a table of 256 rows has work for all 16 waves
+    const uint32_t threads = pieces <= kMinTableThreads / kWave * 4 && pages <= 16384 ? kMinTableThreads : kMaxTableThreads;
+    page_table_kernel<<<markers + fill, threads, lds, st>>>(PageTableArgs{
         out, old, old_stride, want, want_s, page_rows, pages, markers, (uint32_t *)work, arrivals});
     return hipGetLastError();
 }
@@ -342,29 +345,37 @@ template <typename T, int HALF> __global__ __launch_bounds__(256) void update_pa
     __shared__ float2 cs[kPagedMaxHd / 2];
     const uint32_t tok = blockIdx.x, t = threadIdx.x;
     const uint32_t slot = a.map[(size_t)tok * a.map_s], pos = a.map[(size_t)tok * a.map_s + 1];
-    const uint32_t R = a.cache.n[2], hd = a.cache.n[3], KV = a.cache.n[1] / 2, page = slot / R;
+    const uint32_t R = a.cache.n[2], hd = a.cache.n[3], KV = a.cache.n[1] / 2;
+    const int style = a.rope.style;
+    const uint32_t per = hd / (2 * HALF), end = min(2 * KV * per, (blockIdx.y + 1) * a.units);
+    const double turns = t < hd / 2 ? a.rope.turns[t] : 0.0;
+    uint32_t u = blockIdx.y * a.units + t, h, d0, d1;
+    bool halves;
+    float x[HALF], y[HALF];
+    auto load = [&]() {
+        h = u / per;
+        halves = style == 2 && h < KV;
+        d0 = HALF * (halves ? u % per : 2 * (u % per));
+        d1 = d0 + (halves ? hd / 2 : HALF);
+        const TView &src = h < KV ? a.k : a.v;
+        const T *from = (const T *)src.p + (size_t)tok * src.s[1] + (size_t)(h < KV ? h : h - KV) * src.s[2];
+        load_n<T, HALF>(from + (size_t)d0 * src.s[3], src.s[3], a.vec, x);
+        load_n<T, HALF>(from + (size_t)d1 * src.s[3], src.s[3], a.vec, y);
+    };
+    if (u < end)
+        load(); // on its way while the slot and the rotations are
+    const uint32_t page = slot / R;
     if (page >= a.cache.n[0])
         return;
-    const int style = a.rope.style;
     if (style)
     {
         if (t < hd / 2)
-            cs[t] = turn_at(pos, a.rope.turns[t]);
-        __syncthreads();
+            cs[t] = turn_at(pos, turns);
+        lds_barrier();
     }
-    const uint32_t per = hd / (2 * HALF), all = 2 * KV * per;
     T *to = (T *)a.cache.p + (size_t)page * a.cache.s[0] + (size_t)(slot % R) * hd;
-    for (uint32_t u = blockIdx.y * a.units + t; u < min(all, (blockIdx.y + 1) * a.units); u += 256)
+    while (u < end)
     {
-        const uint32_t h = u / per, c = u % per;
-        const TView &src = h < KV ? a.k : a.v;
-        const T *from = (const T *)src.p + (size_t)tok * src.s[1] + (size_t)(h < KV ? h : h - KV) * src.s[2];
-        T *row = to + (size_t)h * a.cache.s[1];
-        const bool halves = style == 2 && h < KV;
-        const uint32_t d0 = HALF * (halves ? c : 2 * c), d1 = d0 + (halves ? hd / 2 : HALF);
-        float x[HALF], y[HALF];
-        load_n<T, HALF>(from + (size_t)d0 * src.s[3], src.s[3], a.vec, x);
-        load_n<T, HALF>(from + (size_t)d1 * src.s[3], src.s[3], a.vec, y);
         if (halves)
         {
 #pragma unroll
@@ -391,8 +402,12 @@ template <typename T, int HALF> __global__ __launch_bounds__(256) void update_pa
             turn(x, d0 / 2);
             turn(y, d1 / 2);
         }
+        T *row = to + (size_t)h * a.cache.s[1];
         store_n<T, HALF>(row + d0, x);
         store_n<T, HALF>(row + d1, y);
+        u += 256;
+        if (u < end)
+            load();
     }
 }
 

@@ -70,10 +70,29 @@ static vk::PagedRope rope_of(float base, bool neox, uint32_t hd)
     return r;
 }
 
+// Memory that a first call makes cannot be made while the context's stream is captured into a hipGraph: the call is refused
+// and the capture goes on
+static vkllm_err_t may_allocate(vkllm_context *context, const char *what)
+{
+    hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+    HIP_TRY(hipStreamIsCapturing(context->device->stream, &status));
+    if (status == hipStreamCaptureStatusNone)
+        return VKLLM_ERR_OK;
+    log_error("%s has no memory yet: run it once before the stream is captured", what);
+    return VKLLM_ERR_ARGS;
+}
+
+static vkllm_err_t output_memory(vkllm_context *context, vkllm_tensor *tensor)
+{
+    return tensor_base(tensor)->data.dev ? VKLLM_ERR_OK : may_allocate(context, tensor->name);
+}
+
 // The context's workspace and arrival counters, made at the first use and kept until the context is freed
 static vkllm_err_t paged_memory(vkllm_context *context, float **work, size_t *work_elems)
 {
     vkllm_gpu_device *dev = context->device;
+    if (!dev->op_work || !dev->paged_arrivals)
+        _CHECK(may_allocate(context, "the operators' workspace"));
     _CHECK(op_workspace(context, work, work_elems));
     if (!*work)
         return VKLLM_ERR_ALLOC;
@@ -127,6 +146,7 @@ extern "C" vkllm_err_t vkllm_op_page_table_run(struct vkllm_context *context, st
     if (tensor->srcs[1])
         CHECK_VIEW(tensor->srcs[1]);
     CHECK_VIEW(tensor);
+    _CHECK(output_memory(context, tensor));
     vkllm_op_page_table_params p;
     memcpy(&p, tensor->params, sizeof(p));
     vk::TView want = tview(context, tensor->srcs[0]), out = tview(context, tensor), old{};
@@ -167,6 +187,8 @@ extern "C" vkllm_err_t vkllm_op_slot_map_init(struct vkllm_context *context, str
     const vkllm_tensor *table = tensor->srcs[0];
     _CHECK_ARGS(is_page_table(table));
     _CHECK_ARGS(word_list(tensor->srcs[1], table->shapes[2]) && word_list(tensor->srcs[2], table->shapes[2]));
+    for (int i = 0; i < 3; ++i)
+        _CHECK_ARGS(!same_memory(tensor, tensor->srcs[i]));
     vkllm_op_slot_map_params p;
     memcpy(&p, tensor->params, sizeof(p));
     _CHECK_ARGS(p.page_rows > 0);
@@ -182,6 +204,7 @@ extern "C" vkllm_err_t vkllm_op_slot_map_run(struct vkllm_context *context, stru
     for (int i = 0; i < 3; ++i)
         CHECK_VIEW(tensor->srcs[i]);
     CHECK_VIEW(tensor);
+    _CHECK(output_memory(context, tensor));
     vkllm_op_slot_map_params p;
     memcpy(&p, tensor->params, sizeof(p));
     vk::TView table = tview(context, tensor->srcs[0]), lengths = tview(context, tensor->srcs[1]),
@@ -239,6 +262,7 @@ extern "C" vkllm_err_t vkllm_op_update_pages_run(struct vkllm_context *context, 
     for (int i = 0; i < 3; ++i)
         CHECK_VIEW(tensor->srcs[i]);
     CHECK_VIEW(tensor);
+    _CHECK(output_memory(context, tensor));
     vkllm_op_update_pages_params p;
     memcpy(&p, tensor->params, sizeof(p));
     vk::TView k = tview(context, tensor->srcs[0]), v = tview(context, tensor->srcs[1]),
@@ -281,6 +305,7 @@ extern "C" vkllm_err_t vkllm_op_paged_attn_init(struct vkllm_context *context, s
     _CHECK_ARGS(is_paged_cache(cache) && cache->shapes[2] % 16 == 0 && cache->shapes[3] == q->shapes[3]);
     _CHECK_ARGS(q->shapes[2] % (cache->shapes[1] / 2) == 0);
     _CHECK_ARGS(is_page_table(table) && table->shapes[2] == q->shapes[1]);
+    _CHECK_ARGS((uint64_t)(table->shapes[3] - 1) * cache->shapes[2] <= 1ull << 31);
     _CHECK_ARGS(!same_memory(tensor, q) && !same_memory(tensor, cache) && !same_memory(tensor, table));
     vkllm_op_paged_attn_params p;
     memcpy(&p, tensor->params, sizeof(p));
@@ -300,6 +325,7 @@ extern "C" vkllm_err_t vkllm_op_paged_attn_run(struct vkllm_context *context, st
     for (int i = 0; i < 3; ++i)
         CHECK_VIEW(tensor->srcs[i]);
     CHECK_VIEW(tensor);
+    _CHECK(output_memory(context, tensor));
     vkllm_op_paged_attn_params p;
     memcpy(&p, tensor->params, sizeof(p));
     vk::TView q = tview(context, tensor->srcs[0]), cache = tview(context, tensor->srcs[1]),
@@ -374,6 +400,7 @@ extern "C" vkllm_err_t vkllm_op_adjust_logits_run(struct vkllm_context *context,
         }
     }
     CHECK_VIEW(tensor);
+    _CHECK(output_memory(context, tensor));
     vk::TView x = tview(context, tensor->srcs[0]), out = tview(context, tensor);
     NEED_DEV(x);
     NEED_DEV(out);
