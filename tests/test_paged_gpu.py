@@ -277,8 +277,17 @@ ATTN = [  # lengths, H, KV, hd, R, base, neox, view
     ([9000, 1, 0, 12345], 8, 8, 64, 16, 1e4, False, None),
     ([3] * 300 + [0] * 20 + [400] * 5, 4, 2, 64, 16, 1e4, False, None),  # more rows than threads
     ([60000, 5], 16, 1, 64, 32, 1e4, False, None),          # joined over three levels, 16 heads a part
-    ([50000, 0, 30], 1, 1, 128, 16, 1e4, True, None),       # and with several threads to a pair of dims
+    ([50000, 0, 30], 1, 1, 128, 16, 1e4, True, None),       # and with several threads to the same dims
     ([700] * 65 + [0, 3000], 6, 3, 48, 16, 1e4, False, None),  # several rows to a workgroup, starts and ends counted
+    # joins in which 8, 4, 2 lanes and one thread have four dims, and a thread eight
+    ([7000], 2, 1, 16, 16, 1e4, True, None),
+    ([6000, 1], 3, 1, 72, 32, 1e4, False, None),
+    ([8000], 4, 1, 64, 16, 1e4, False, None),
+    ([5000], 10, 2, 96, 16, 1e4, True, None),
+    ([9000, 0], 9, 1, 128, 64, 1e4, False, None),
+    ([4000, 10], 5, 1, 256, 16, 1e4, True, None),
+    ([3000], 12, 1, 200, 16, 1e4, False, None),
+    ([30000], 11, 1, 120, 64, 0.0, False, None),
 ]
 
 

@@ -29,8 +29,9 @@ typedef _Float16 half8 __attribute__((ext_vector_type(8)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kHeadsPerTile = 16;
-// what starting and ending a (sequence, head) costs a workgroup, in units: 64 ragged rows of up to 8192 over 8 key heads
-// of 128 took 121 us with 0 and 117 with 1 (workgroups with many short rows had ended last)
+// What starting and ending a (sequence, head) costs a workgroup, in units (workgroups with many short rows ended last).
+// fp16, us with 0 / 1 / 2: 70 ragged rows of up to 8192 over 9 key heads of 64 80 / 74 / 74, 30 over 5 of 256 86 / 79 / 80,
+// 200 of up to 500 over 9 of 128 34 / 36 / 37
 constexpr uint32_t kSegmentUnits = 1;
 constexpr float kNegInf = -INFINITY;
 
@@ -71,12 +72,20 @@ __device__ __forceinline__ float2 get2(const float *p)
     return {__uint_as_float((uint32_t)v), __uint_as_float((uint32_t)(v >> 32))};
 }
 
-// A thread joins kJoinFan parts of two dims. Where a part has fewer than 256 pairs of dims, several threads share a pair.
-constexpr uint32_t kJoinFan = 8, kJoinLevels = 4; // 8^4 parts
-__device__ __forceinline__ uint32_t join_ways(uint32_t pairs)
+// A thread joins kJoinFan parts of four dims (of eight, loads of both in flight, where a part has more than 256 fours).
+// Where it has 128 or fewer, 2, 4 or 8 lanes share a four, so a level takes up to 64 parts. One row of 2000 positions, us
+// against pairs of dims and no lanes that share by shuffles: 16 heads on 1 key head 14.8 for 27, 32 on 8 9.5 for 13.1.
+constexpr uint32_t kJoinFan = 8, kJoinLevels = 4;
+static_assert(1u << 3 * kJoinLevels >= kPagedMaxWorkgroups && kPagedArrivals == 2 * kJoinLevels * kPagedMaxWorkgroups);
+__device__ __forceinline__ uint32_t join_ways(uint32_t fours)
 {
-    return pairs >= 256 ? 1 : min(8u, 256 / pairs);
+    return fours > 128 ? 1 : fours > 64 ? 2 : fours > 32 ? 4 : 8;
 }
+struct Joined
+{
+    float m, l;
+    f32x4 o;
+};
 
 template <bool F16, int HDP> struct PagedTile
 {
@@ -91,8 +100,9 @@ template <bool F16, int HDP> struct PagedTile
     // and the matrix cores have the time
     static constexpr int QN = F16 ? 2 : 1;
     static constexpr int NP = kHeadsPerTile * HDP / 2 / 256; // query pairs that a thread stages
-    // Workgroups per CU. fp16, us with 1 / 2 / 3: 50 rows of up to 8192 over 5 key heads of 128 57 / 59 / 66, 200 rows of up
-    // to 500 over 9 39 / 36 / 43, 30 rows of up to 8192 over 5 of 256 82 / 94 / 103, 70 rows over 9 of 64 73 / 75 / 76
+    // Workgroups per CU. fp16, us with 1 / 2 / 3: 50 rows of up to 8192 over 5 key heads of 128 56 / 58 / 64, 200 rows of up
+    // to 500 over 9 39 / 36 / 42, 30 rows of up to 8192 over 5 of 256 79 / 87 / 97, 70 rows over 9 of 64 72 / 74 / 83, one
+    // row of 8000 over 8 of 128 18.6 / 15.5 / 15.6
     static constexpr int PER_CU = HDP == 256 ? 1 : 2;
 };
 
@@ -107,7 +117,7 @@ __device__ __forceinline__ float exp2_of(float x)
     return __builtin_amdgcn_exp2f(x);
 }
 
-// dynamic LDS: lengths [B], queries [QN][16][QP], per-wave statistics [4][16][2], per-wave sums [4][tile_heads][hd]
+// dynamic LDS, aligned for the 16-byte accesses (1 to 2 us per launch): lengths [B], queries [QN][16][QP], per-wave statistics [4][16][2], per-wave sums [4][tile_heads][hd]
 // FULL: head_dim is HDP, else it is smaller
 template <bool F16, int HDP, bool FULL>
 __global__ __launch_bounds__(256, HDP == 256 ? 1 : 2) void paged_attn_kernel(PagedAttnArgs a)
@@ -117,10 +127,9 @@ __global__ __launch_bounds__(256, HDP == 256 ? 1 : 2) void paged_attn_kernel(Pag
     constexpr int NT = Tile::NT, KW = Tile::KW, KT = Tile::KT, KS = Tile::KS, VD = Tile::VD, VW = Tile::VW,
                   QP = Tile::QP, QN = Tile::QN, NP = Tile::NP;
     constexpr uint32_t ES = sizeof(T);
-    extern __shared__ uint32_t lds[];
+    extern __shared__ __align__(16) uint32_t lds[];
     __shared__ uint64_t scan[4], first_unit;
     __shared__ uint32_t first_row, arrived;
-    __shared__ f32x4 joined[256];
     // the rows whose parts lie in slots 0 and 1: how many parts they have, and the number of this one
     struct Split
     {
@@ -639,8 +648,8 @@ __global__ __launch_bounds__(256, HDP == 256 ? 1 : 2) void paged_attn_kernel(Pag
         const uint32_t head0 = __builtin_amdgcn_readfirstlane(split[which].head0),
                        Gn = __builtin_amdgcn_readfirstlane(split[which].heads);
         uint32_t k = __builtin_amdgcn_readfirstlane(split[which].number), stride = 1;
-        const uint32_t first = blockIdx.x - k, pairs = Gn * (HDP / 2);
-        const uint32_t ways = join_ways(pairs), fan = kJoinFan * ways;
+        const uint32_t first = blockIdx.x - k, fours = Gn * (HDP / 4);
+        const uint32_t ways = join_ways(fours), fan = kJoinFan * ways;
         const uint32_t floats = part_floats(a.tile_heads, hd), half = 2 * gridDim.x * floats; // of 2^26 at most
         // the place of part k: the first part's row starts in its workgroup, the others' does not
         auto slot = [&](uint32_t k) { return 2 * (first + k) + (k == 0 ? 1 : 0); };
@@ -662,74 +671,89 @@ __global__ __launch_bounds__(256, HDP == 256 ? 1 : 2) void paged_attn_kernel(Pag
             // levels write one half of the workspace and read the other, so nothing is overwritten that is still read
             const float *in = a.parts + (level % 2) * half;
             float *to = a.parts + (1 - level % 2) * half + slot(lead) * floats;
-            // (m, l, o, o) of pair e from parts way, way + ways, ... of the group (dims past the head repeat its last)
-            auto gather = [&](uint32_t e, uint32_t way) {
-                float2 o[kJoinFan], ml[kJoinFan];
-                const uint32_t i = e / (HDP / 2), d = min(e % (HDP / 2) * 2, hd - 2);
+            // fours e, e + 256, ... from parts way, way + ways, ... of the group (what lies past it repeats its last)
+            auto gather = [&](auto count, Joined *r, uint32_t e, uint32_t way) {
+                constexpr int N = decltype(count)::value;
+                float2 o[N][kJoinFan][2], ml[N][kJoinFan];
 #pragma unroll
-                for (uint32_t c = 0; c < kJoinFan; ++c)
+                for (int j = 0; j < N; ++j)
                 {
-                    const float *part = in + slot(lead + min(way + c * ways, size - 1) * stride) * floats;
-                    o[c] = get2(part + i * hd + d);
-                    ml[c] = get2(part + a.tile_heads * hd + 2 * i);
-                }
-                float m = kNegInf;
+                    const uint32_t f = min(e + 256 * j, fours - 1), i = f / (HDP / 4), d = min(f % (HDP / 4) * 4, hd - 4);
 #pragma unroll
-                for (uint32_t c = 0; c < kJoinFan; ++c)
-                {
-                    if (way + c * ways >= size)
-                        ml[c].x = kNegInf;
-                    m = fmaxf(m, ml[c].x);
+                    for (uint32_t c = 0; c < kJoinFan; ++c)
+                    {
+                        o[j][c][0] = o[j][c][1] = ml[j][c] = {0.f, 0.f};
+                        if (c * ways >= size)
+                            continue;
+                        const float *part = in + slot(lead + min(way + c * ways, size - 1) * stride) * floats;
+                        o[j][c][0] = get2(part + i * hd + d);
+                        o[j][c][1] = get2(part + i * hd + d + 2);
+                        ml[j][c] = get2(part + a.tile_heads * hd + 2 * i);
+                    }
                 }
-                f32x4 r = {m, 0.f, 0.f, 0.f};
 #pragma unroll
-                for (uint32_t c = 0; c < kJoinFan; ++c)
+                for (int j = 0; j < N; ++j)
                 {
-                    // a part without a largest score counts with 0, which keeps a sum that is not a number one
-                    const float f = ml[c].x == kNegInf ? 0.f : exp2_of(ml[c].x - m);
-                    r[1] += f * ml[c].y;
-                    r[2] += f * o[c].x;
-                    r[3] += f * o[c].y;
+                    Joined x = {kNegInf, 0.f, {0.f, 0.f, 0.f, 0.f}};
+#pragma unroll
+                    for (uint32_t c = 0; c < kJoinFan; ++c)
+                    {
+                        if (way + c * ways >= size)
+                            ml[j][c].x = kNegInf;
+                        x.m = fmaxf(x.m, ml[j][c].x);
+                    }
+#pragma unroll
+                    for (uint32_t c = 0; c < kJoinFan; ++c)
+                    {
+                        // a part without a largest score counts with 0, which keeps a sum that is not a number one
+                        const float f = ml[j][c].x == kNegInf ? 0.f : exp2_of(ml[j][c].x - x.m);
+                        x.l += f * ml[j][c].y;
+                        x.o += f * (f32x4){o[j][c][0].x, o[j][c][0].y, o[j][c][1].x, o[j][c][1].y};
+                    }
+                    r[j] = x;
                 }
-                return r;
             };
-            auto emit = [&](uint32_t e, f32x4 r) {
-                const uint32_t i = e / (HDP / 2), d = e % (HDP / 2) * 2;
-                if (!FULL && d >= hd)
+            auto emit = [&](uint32_t e, const Joined &r) {
+                const uint32_t i = e / (HDP / 4), d = e % (HDP / 4) * 4;
+                if (e >= fours || (!FULL && d >= hd))
                     return;
                 if (n <= fan)
-                    store_out(split[which].b, head0 + i, d, r[2], r[3], r[1]);
+                {
+                    store_out(split[which].b, head0 + i, d, r.o[0], r.o[1], r.l);
+                    store_out(split[which].b, head0 + i, d + 2, r.o[2], r.o[3], r.l);
+                }
                 else
                 {
-                    put2(to + i * hd + d, r[2], r[3]);
+                    put2(to + i * hd + d, r.o[0], r.o[1]);
+                    put2(to + i * hd + d + 2, r.o[2], r.o[3]);
                     if (d == 0)
-                        put2(to + a.tile_heads * hd + 2 * i, r[0], r[1]);
+                        put2(to + a.tile_heads * hd + 2 * i, r.m, r.l);
                 }
             };
             if (ways == 1)
-                for (uint32_t e = t; e < pairs; e += 256)
-                    emit(e, gather(e, 0));
+                for (uint32_t e = t; e < fours; e += 512)
+                {
+                    Joined r[2];
+                    gather(std::integral_constant<int, 2>(), r, e, 0);
+                    emit(e, r[0]);
+                    emit(e + 256, r[1]);
+                }
             else
             {
-                if (t < ways * pairs)
-                    joined[t] = gather(t % pairs, t / pairs);
-                __syncthreads();
-                if (t < pairs)
+                Joined r;
+                gather(std::integral_constant<int, 1>(), &r, t / ways, t % ways);
+                for (uint32_t w = 1; w < ways; w *= 2)
                 {
-                    float m = kNegInf;
-                    for (uint32_t w = 0; w < ways; ++w)
-                        m = fmaxf(m, joined[w * pairs + t][0]);
-                    f32x4 r = {m, 0.f, 0.f, 0.f};
-                    for (uint32_t w = 0; w < ways; ++w)
-                    {
-                        const f32x4 x = joined[w * pairs + t];
-                        const float f = x[0] == kNegInf ? 0.f : exp2_of(x[0] - m);
-                        r[1] += f * x[1];
-                        r[2] += f * x[2];
-                        r[3] += f * x[3];
-                    }
-                    emit(t, r);
+                    const float m = __shfl_xor(r.m, w, kWave), l = __shfl_xor(r.l, w, kWave), top = fmaxf(r.m, m);
+                    const float f = r.m == kNegInf ? 0.f : exp2_of(r.m - top), h = m == kNegInf ? 0.f : exp2_of(m - top);
+                    r.m = top;
+                    r.l = f * r.l + h * l;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        r.o[i] = f * r.o[i] + h * __shfl_xor(r.o[i], w, kWave);
                 }
+                if (t % ways == 0)
+                    emit(t / ways, r);
             }
             if (n <= fan)
                 break;
