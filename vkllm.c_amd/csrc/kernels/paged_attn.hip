@@ -117,7 +117,8 @@ __device__ __forceinline__ float exp2_of(float x)
     return __builtin_amdgcn_exp2f(x);
 }
 
-// dynamic LDS, aligned for the 16-byte accesses (1 to 2 us per launch): lengths [B], queries [QN][16][QP], per-wave statistics [4][16][2], per-wave sums [4][tile_heads][hd]
+// dynamic LDS, aligned for 16-byte accesses (left to chance, launches took 1 to 2 us more): lengths [B], queries
+// [QN][16][QP], per-wave statistics [4][16][2], per-wave sums [4][tile_heads][hd]
 // FULL: head_dim is HDP, else it is smaller
 template <bool F16, int HDP, bool FULL>
 __global__ __launch_bounds__(256, HDP == 256 ? 1 : 2) void paged_attn_kernel(PagedAttnArgs a)
@@ -166,8 +167,18 @@ __global__ __launch_bounds__(256, HDP == 256 ? 1 : 2) void paged_attn_kernel(Pag
     uint32_t row0;                // the first row
     auto weigh = [&](uint64_t sum) { return ((sum & ((1ull << 40) - 1)) + extra * (sum >> 40)) * heads; };
     auto divide = [&](uint64_t total) {
-        extra = (total & ((1ull << 40) - 1)) * heads > 4 * gridDim.x ? kSegmentUnits : 0;
-        share = quotient(weigh(total) + gridDim.x - 1, gridDim.x);
+        // Long rows of 128 dims go to half of the workgroups, one per CU, the others end here: a unit's 64 KB per CU on their
+        // way are enough, and no older workgroup runs ahead of a younger one beside it and leaves it the end. Short rows want
+        // the second one's loads meanwhile; few units of few rows would have fewer loads on their way, for the same joins.
+        // us with all / half of them: 2 rows of up to 131072 on 4 key heads 76.7 / 71, 1 of 3000 on 32 16.1 / 14.2, 2 of 1100
+        // 18.3 / 13, 50 ragged ones of up to 8192 on 5 58 / 56, and fp32 60 / 58.5; but 64 of 8192 on 8 358 / 360 (fp32, of 768,
+        // 72 / 74), and kept out 1 of 12000 on 8 18.5 / 20.6, 2048 of 100 196 / 216, 64 of 1024 on 8 of 64 dims 27 / 36.
+        const uint64_t units = (total & ((1ull << 40) - 1)) * heads, rows = (total >> 40) * heads;
+        const uint32_t n = gridDim.x;
+        const bool alone = FULL && HDP == 128 && units >= 6 * rows && (units >= 4 * n || (units > n && 16 * rows >= n));
+        const uint32_t sharers = alone ? (n + 1) / 2 : n;
+        extra = units > 4 * n ? kSegmentUnits : 0;
+        share = quotient(weigh(total) + sharers - 1, sharers);
         u0 = blockIdx.x * share;
         u1 = min(u0 + share, weigh(total));
     };
@@ -396,8 +407,8 @@ __global__ __launch_bounds__(256, HDP == 256 ? 1 : 2) void paged_attn_kernel(Pag
     };
     uint32_t q_at = c * QP + (F16 ? 8 : 4) * g;
 
-    // One unit; `more`: with the loads of the unit `next` (and the pages of the one `after` it). The last unit is code of its own, because
-    // where paths with and without newer loads meet, the compiler waits for all of them.
+    // One unit; `more`: with the loads of the unit `next` (and the pages of the one `after` it). The last unit is code of its
+    // own, because where paths with and without newer loads meet, the compiler waits for all of them.
     auto step = [&](auto more, const Place &next, const Place &after) {
         constexpr bool MORE = decltype(more)::value;
         // read again at every step (the compiler is kept from moving that out of the loop): in registers the queries would
