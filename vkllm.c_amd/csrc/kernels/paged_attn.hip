@@ -72,9 +72,10 @@ __device__ __forceinline__ float2 get2(const float *p)
     return {__uint_as_float((uint32_t)v), __uint_as_float((uint32_t)(v >> 32))};
 }
 
-// A thread joins kJoinFan parts of four dims (of eight, loads of both in flight, where a part has more than 256 fours).
+// A thread joins kJoinFan parts of four dims (of eight, loads of both on their way, where a part has more than 256 fours).
 // Where it has 128 or fewer, 2, 4 or 8 lanes share a four, so a level takes up to 64 parts. One row of 2000 positions, us
-// against pairs of dims and no lanes that share by shuffles: 16 heads on 1 key head 14.8 for 27, 32 on 8 9.5 for 13.1.
+// against pairs of dims joined through LDS: 16 heads on 1 key head 14.8 for 27, 32 on 8 9.5 for 13.1. 16 parts a thread
+// took 0.5 to 2 us more nearly everywhere: a level's cost is the round trip and the code's way to the CU.
 constexpr uint32_t kJoinFan = 8, kJoinLevels = 4;
 static_assert(1u << 3 * kJoinLevels >= kPagedMaxWorkgroups && kPagedArrivals == 2 * kJoinLevels * kPagedMaxWorkgroups);
 __device__ __forceinline__ uint32_t join_ways(uint32_t fours)
@@ -741,7 +742,7 @@ __global__ __launch_bounds__(256, HDP == 256 ? 1 : 2) void paged_attn_kernel(Pag
                         put2(to + a.tile_heads * hd + 2 * i, r.m, r.l);
                 }
             };
-            if (ways == 1)
+            if (fours > 256)
                 for (uint32_t e = t; e < fours; e += 512)
                 {
                     Joined r[2];
