@@ -9,7 +9,8 @@
  *     n > 0:                 y = (x > 0 ? x / repetition : x * repetition) - (frequency * n + presence)
  *     a bias for the token:  y += value (its last one, if it has several)
  *     not allowed:           y = -inf, whatever x is
- * in 32 bits, rounded once. Tokens at or past V are ignored; counts end at the row's width. */
+ * in 32 bits, rounded once. Tokens at or past V are ignored; counts end at the row's width. No source lies
+ * in the tensor's memory. */
 #ifndef VKLLM_OP_ADJUST_LOGITS_H
 #define VKLLM_OP_ADJUST_LOGITS_H
 #include <stdbool.h>

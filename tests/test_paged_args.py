@@ -176,6 +176,15 @@ def test_adjust_logits_refuses(vk, world, kw):
     assert world.init("adjust_logits", adjust(world, **kw)) == vk.ERR_ARGS
 
 
+def test_adjust_logits_refuses_shared_memory(vk, world):
+    for i in range(4):
+        t = adjust(world)
+        view = world.tensor(tuple(t.contents.srcs[i].contents.shapes), t.contents.srcs[i].contents.dtype, vk.OP_REF, [t])
+        view.contents.data.is_ref = True
+        t.contents.srcs[i] = view
+        assert world.init("adjust_logits", t) == vk.ERR_ARGS
+
+
 def test_a_node_of_another_operator_and_missing_arguments(vk, world):
     make = {"page_table": page_table, "slot_map": slot_map, "update_pages": update_pages, "paged_attn": paged_attn,
             "adjust_logits": adjust}

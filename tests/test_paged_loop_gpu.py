@@ -264,3 +264,27 @@ def test_a_first_call_under_capture_is_refused(ctx, vk):
         want, off = attention(q[0], cache, table, 0.125, 0.0, False)
         assert (np.abs(ctx.download(t)[0] - want) <= np.abs(want) * 2.0 ** -11 * 1.001 + off + 2.0 ** -25).all()
         assert np.array_equal(ctx.download(y), ctx.download(x))
+
+
+def test_a_source_that_never_ran_is_refused_under_capture(ctx, vk):
+    """Nor can an operator make the memory of a source: a table that no call has written yet."""
+    H, L = _hip_runtime(), vk.lib()
+    stream, graph = ctypes.c_void_p(), ctypes.c_void_p()
+    vk.check("stream", L.vkllm_hip_context_stream(ctx.vp, ctypes.byref(stream)))
+    with Bag(ctx) as bag:
+        lengths, counts = bag.put(rows4(np.array([[5, 20]], np.uint32))), bag.put(rows4(np.array([[1, 2]], np.uint32)))
+        table = ctx.tensor([1, 1, 2, 4], vk.U32, op=vk.OP_PAGE_TABLE, srcs=[lengths], params=vk.PageTableParams(16, 4))
+        slots = ctx.tensor([1, 1, 3, 2], vk.U32, op=vk.OP_SLOT_MAP, srcs=[table, lengths, counts],
+                           params=vk.SlotMapParams(16))
+        bag.made += [table, slots]
+        ctx.upload(slots, np.zeros((1, 1, 3, 2), np.uint32))
+        assert H.hipStreamBeginCapture(stream, 0) == 0
+        rc = L.vkllm_op_slot_map_run(ctx.vp, ctx.cmds, slots)
+        assert H.hipStreamEndCapture(stream, ctypes.byref(graph)) == 0
+        if graph.value:
+            H.hipGraphDestroy(graph)
+        assert rc == vk.ERR_ARGS
+        ctx.upload(table, np.array([[[[0, 0, 0, 0], [0, 0, 0, 0]]]], np.uint32))
+        vk.check("page_table", ctx.run_op("page_table", table))
+        vk.check("slot_map", ctx.run_op("slot_map", slots))
+        assert ctx.download(slots)[0, 0].tolist() == [[4, 4], [34, 18], [35, 19]]

@@ -1,12 +1,12 @@
 // VKLLM_OP_ADJUST_LOGITS: penalties for used tokens, token biases and a grammar's mask. No counterpart in the reference.
 //
-// A workgroup takes tiles of one row's vocabulary, 32 bytes of logits a thread. It counts the tile's tokens in the row's history and
-// notes their last bias in LDS (whole numbers and a maximum of entry numbers, so the order of the atomics changes
-// nothing), and passes over the logits once, looking every token up. Bound by HBM for batches, by latency for a row.
+// A workgroup takes tiles of one row's vocabulary, 32 bytes of logits a thread. It counts the tile's tokens in the row's
+// history and notes their last bias in LDS (whole numbers and a maximum of entry numbers, so the order of the atomics
+// changes nothing), and passes over the logits once, looking every token up. Bound by HBM for batches, by latency for a row.
 // Tiles are as large as still fill the GPU, since each goes through the row's history; a workgroup with several keeps its
 // share of the history in registers and has the next tile's logits on their way while it works on one. 256 rows of 131072
-// fp16 logits, 4096 used tokens, 300 biases and a mask: a tile per workgroup 47 us, 35 now
-// (4.1 TB/s); with nothing to look up 26.
+// fp16 logits, 4096 used tokens, 300 biases and a mask: a tile per workgroup 47 us, 34 now (4.2 TB/s); with nothing to look
+// up 26.
 #include <algorithm>
 
 #include "device_common.h"

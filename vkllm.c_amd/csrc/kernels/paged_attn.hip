@@ -11,8 +11,9 @@
 // and whichever workgroup of a group of them is the last to arrive joins the group's, up a tree. A workgroup finds
 // its units from prefix sums of the lengths, formed in LDS.
 //
-// Matrix cores do the products although 16 - G of their 16 columns are idle when G heads share a key head: they have 24
-// times the rate that the cache arrives at, and the layout spares the shuffles that dot products of single rows need.
+// Matrix cores do the products although 16 - G of their 16 columns are idle when G heads share a key head: they have 12
+// times the rate that the cache arrives at (fp16, operands in two parts; fp32 3 times), and the layout spares the shuffles
+// that dot products of single rows need.
 // Scores are K Q^T: a wave's 16 keys x 16 heads, of which lane l gets keys 4 (l / 16) + 0..3 of head l % 16. That is, with
 // the contraction numbered accordingly, the operand layout of V^T P^T, so probabilities stay in their lanes. V^T
 // wants several keys of one dim in a lane: a lane loads HDP / 16 dims of its 4 (8) keys and pairs them up by byte permutes.
@@ -415,7 +416,9 @@ __global__ __launch_bounds__(256, HDP == 256 ? 1 : 2) void paged_attn_kernel(Pag
         // read again at every step (the compiler is kept from moving that out of the loop): in registers the queries would
         // cost half of the resident waves
         asm volatile("" : "+v"(q_at));
-        auto query = [&](int n, int s) { return *(const u32x4 *)(qs + q_at + n * kHeadsPerTile * QP + (F16 ? 32 : 16) * s); };
+        auto query = [&](int n, int s) {
+            return *(const u32x4 *)(qs + q_at + n * kHeadsPerTile * QP + (F16 ? 32 : 16) * s);
+        };
         f32x4 x[NT];
 #pragma unroll
         for (int i = 0; i < NT; ++i)

@@ -301,8 +301,9 @@ hipError_t launch_slot_map(hipStream_t st, const PageTableView &table, const uin
 }
 
 // ---------------------------------------------------------------------------------------------------------------
-// VKLLM_OP_UPDATE_PAGES. A workgroup has one token (or a share of its heads): the rotations of its position go
-// into LDS once, then a thread moves units of a head: neighbouring elements, or for pairs of halves as many of both. Bound by HBM for prompts, by latency for a token.
+// VKLLM_OP_UPDATE_PAGES. A workgroup has one token (or a share of its heads): the rotations of its position go into LDS
+// once, then a thread moves units of a head: neighbouring elements, or for pairs of halves as many of both. Bound by HBM for
+// prompts, by latency for a token.
 struct UpdatePagesArgs
 {
     TView cache, k, v;
@@ -418,7 +419,7 @@ hipError_t launch_update_pages(hipStream_t st, const TView &cache, const TView &
         return t.s[3] == 1 && t.s[2] % 8 == 0 && t.s[1] % 8 == 0 && (uintptr_t)t.p % 16 == 0;
     };
     // 16 bytes of each half where heads allow it (a thread then moves 32); us for 4001 tokens of 32 key heads of 128 in fp16,
-    // pairs of halves: 8 bytes 31.2, 16 29.8 (28.0 on the GPU, 4.7 TB/s: a large copy's rate is 4.9)
+    // pairs of halves: 8 bytes 31.2, 16 27.8 (27.4 on the GPU, 4.8 TB/s: a large copy's rate is 4.9)
     const uint32_t hd = cache.n[3], half = cache.dt == DT_F16 && hd % 16 == 0 ? 8 : 4;
     const uint32_t T = k.n[1], all = cache.n[1] * (hd / (2 * half));
     const uint32_t shares = min((all - 1) / 256 + 1, T >= 1024 ? 1u : (1023 / T) + 1);

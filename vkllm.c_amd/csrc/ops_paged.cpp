@@ -82,9 +82,15 @@ static vkllm_err_t may_allocate(vkllm_context *context, const char *what)
     return VKLLM_ERR_ARGS;
 }
 
-static vkllm_err_t output_memory(vkllm_context *context, vkllm_tensor *tensor)
+// the node's tensor and its sources
+static vkllm_err_t node_memory(vkllm_context *context, vkllm_tensor *tensor)
 {
-    return tensor_base(tensor)->data.dev ? VKLLM_ERR_OK : may_allocate(context, tensor->name);
+    if (!tensor_base(tensor)->data.dev)
+        _CHECK(may_allocate(context, tensor->name));
+    for (vkllm_tensor *src : tensor->srcs)
+        if (src && !tensor_base(src)->data.dev)
+            _CHECK(may_allocate(context, src->name));
+    return VKLLM_ERR_OK;
 }
 
 // The context's workspace and arrival counters, made at the first use and kept until the context is freed
@@ -111,6 +117,7 @@ static vkllm_err_t paged_memory(vkllm_context *context, float **work, size_t *wo
     dev->paged_arrivals = p;
     return VKLLM_ERR_OK;
 }
+
 // =============================================================================================================
 // PAGE_TABLE
 extern "C" vkllm_err_t vkllm_op_page_table_init(struct vkllm_context *context, struct vkllm_commands *commands,
@@ -146,7 +153,7 @@ extern "C" vkllm_err_t vkllm_op_page_table_run(struct vkllm_context *context, st
     if (tensor->srcs[1])
         CHECK_VIEW(tensor->srcs[1]);
     CHECK_VIEW(tensor);
-    _CHECK(output_memory(context, tensor));
+    _CHECK(node_memory(context, tensor));
     vkllm_op_page_table_params p;
     memcpy(&p, tensor->params, sizeof(p));
     vk::TView want = tview(context, tensor->srcs[0]), out = tview(context, tensor), old{};
@@ -204,7 +211,7 @@ extern "C" vkllm_err_t vkllm_op_slot_map_run(struct vkllm_context *context, stru
     for (int i = 0; i < 3; ++i)
         CHECK_VIEW(tensor->srcs[i]);
     CHECK_VIEW(tensor);
-    _CHECK(output_memory(context, tensor));
+    _CHECK(node_memory(context, tensor));
     vkllm_op_slot_map_params p;
     memcpy(&p, tensor->params, sizeof(p));
     vk::TView table = tview(context, tensor->srcs[0]), lengths = tview(context, tensor->srcs[1]),
@@ -262,7 +269,7 @@ extern "C" vkllm_err_t vkllm_op_update_pages_run(struct vkllm_context *context, 
     for (int i = 0; i < 3; ++i)
         CHECK_VIEW(tensor->srcs[i]);
     CHECK_VIEW(tensor);
-    _CHECK(output_memory(context, tensor));
+    _CHECK(node_memory(context, tensor));
     vkllm_op_update_pages_params p;
     memcpy(&p, tensor->params, sizeof(p));
     vk::TView k = tview(context, tensor->srcs[0]), v = tview(context, tensor->srcs[1]),
@@ -286,7 +293,6 @@ extern "C" vkllm_err_t vkllm_op_update_pages_post_run(struct vkllm_context *, st
 
 // =============================================================================================================
 // PAGED_ATTN
-
 extern "C" vkllm_err_t vkllm_op_paged_attn_init(struct vkllm_context *context, struct vkllm_commands *commands,
                                                 struct vkllm_tensor *tensor)
 {
@@ -325,7 +331,7 @@ extern "C" vkllm_err_t vkllm_op_paged_attn_run(struct vkllm_context *context, st
     for (int i = 0; i < 3; ++i)
         CHECK_VIEW(tensor->srcs[i]);
     CHECK_VIEW(tensor);
-    _CHECK(output_memory(context, tensor));
+    _CHECK(node_memory(context, tensor));
     vkllm_op_paged_attn_params p;
     memcpy(&p, tensor->params, sizeof(p));
     vk::TView q = tview(context, tensor->srcs[0]), cache = tview(context, tensor->srcs[1]),
@@ -368,7 +374,8 @@ extern "C" vkllm_err_t vkllm_op_adjust_logits_init(struct vkllm_context *context
         return VKLLM_ERR_ARGS;
     }
     _CHECK_ARGS(x->strides[3] == dtype_bytes(x->dtype) && tensor->strides[3] == dtype_bytes(x->dtype));
-    _CHECK_ARGS(!same_memory(tensor, x));
+    for (vkllm_tensor *src : {x, history, rules, mask})
+        _CHECK_ARGS(!src || !same_memory(tensor, src));
     const uint32_t B = x->shapes[2], V = x->shapes[3];
     _CHECK_ARGS(B <= 65535); // a workgroup row each
     if (history)
@@ -400,7 +407,7 @@ extern "C" vkllm_err_t vkllm_op_adjust_logits_run(struct vkllm_context *context,
         }
     }
     CHECK_VIEW(tensor);
-    _CHECK(output_memory(context, tensor));
+    _CHECK(node_memory(context, tensor));
     vk::TView x = tview(context, tensor->srcs[0]), out = tview(context, tensor);
     NEED_DEV(x);
     NEED_DEV(out);
