@@ -108,10 +108,11 @@ template <bool F16, int HDP> struct PagedTile
     static constexpr int PER_CU = HDP == 256 ? 1 : 2;
 };
 
-// n / d, d > 0, by the much shorter 32-bit division where that is the same
+// n / d, d > 0, for n below 2^52: the double's rounding is then too small to reach the next whole number. Shorter than a
+// division of 64-bit words, of which the code would hold six.
 __device__ __forceinline__ uint64_t quotient(uint64_t n, uint64_t d)
 {
-    return (n | d) >> 32 ? n / d : (uint32_t)n / (uint32_t)d;
+    return (uint64_t)((double)n / (double)d);
 }
 
 __device__ __forceinline__ float exp2_of(float x)
