@@ -288,6 +288,11 @@ ATTN = [  # lengths, H, KV, hd, R, base, neox, view
     ([4000, 10], 5, 1, 256, 16, 1e4, True, None),
     ([3000], 12, 1, 200, 16, 1e4, False, None),
     ([30000], 11, 1, 120, 64, 0.0, False, None),
+    # long rows of 128 dims: a workgroup per CU, with and without starts counted, and more rows than lanes
+    ([1100, 1080], 32, 32, 128, 16, 1e4, True, None),
+    ([1500, 0, 1] + [1490] * 23, 16, 8, 128, 64, 1e4, False, None),
+    ([900] * 68 + [0, 790, 1], 4, 2, 128, 16, 1e4, True, None),
+    ([70000, 3], 8, 4, 128, 16, 1e4, True, None),
 ]
 
 

@@ -288,3 +288,69 @@ def test_a_source_that_never_ran_is_refused_under_capture(ctx, vk):
         vk.check("page_table", ctx.run_op("page_table", table))
         vk.check("slot_map", ctx.run_op("slot_map", slots))
         assert ctx.download(slots)[0, 0].tolist() == [[4, 4], [34, 18], [35, 19]]
+
+
+def test_two_captured_calls_share_the_workspace(ctx, vk):
+    """Two attention calls, one of long rows that are joined over two levels and one of many short rows, each in a graph of its
+    own on the context's stream, replayed in turn with lengths that change between the replays and without a wait between
+    the two: every result is that of an eager call, and so are those of the eager calls behind the replays."""
+    H, L = _hip_runtime(), vk.lib()
+    stream = ctypes.c_void_p()
+    vk.check("stream", L.vkllm_hip_context_stream(ctx.vp, ctypes.byref(stream)))
+    r = np.random.default_rng(21)
+    shapes = [(2, 16, 1, 128, 1200, 16), (70, 4, 2, 64, 12, 16)]  # rows, heads, key heads, head_dim, columns, page rows
+    graphs, execs = [], []
+    with Bag(ctx) as bag:
+        tables, outs = [], []
+        for B, heads, KV, hd, P, R in shapes:
+            pages = 300
+            q = bag.put(r.standard_normal((1, B, heads, hd)).astype(np.float16))
+            cache = bag.put(r.standard_normal((pages, 2 * KV, R, hd)).astype(np.float16))
+            ids = r.integers(0, pages, (B, 1 + P)).astype(np.uint32)  # pages that rows share
+            tables.append((bag.put(rows4(ids)), ids))
+            outs.append(ctx.tensor([1, B, heads, hd], vk.F16, op=vk.OP_PAGED_ATTN, srcs=[q, cache, tables[-1][0]],
+                                   params=vk.PagedAttnParams(hd ** -0.5, 1e4, True)))
+            bag.made.append(outs[-1])
+
+        def set_lengths(i):
+            for (t, ids), (B, _, _, _, P, R) in zip(tables, shapes):
+                lengths = np.random.default_rng(100 + i).integers(0, P * R + 1, B)
+                lengths[-1] = P * R if i % 2 else 0
+                ids[:, 0] = lengths
+                ctx.upload(t, rows4(ids))
+
+        def eager():
+            for t in outs:
+                vk.check("paged_attn", L.vkllm_op_paged_attn_run(ctx.vp, ctx.cmds, t))
+            return [ctx.download_raw(t).copy() for t in outs]
+
+        want = []
+        for i in range(5):
+            set_lengths(i)
+            want.append(eager())
+        try:
+            for t in outs:
+                graphs.append(ctypes.c_void_p())
+                execs.append(ctypes.c_void_p())
+                assert H.hipStreamBeginCapture(stream, 0) == 0
+                rc = L.vkllm_op_paged_attn_run(ctx.vp, ctx.cmds, t)
+                end = H.hipStreamEndCapture(stream, ctypes.byref(graphs[-1]))
+                assert rc == vk.ERR_OK and end == 0
+                assert H.hipGraphInstantiate(ctypes.byref(execs[-1]), graphs[-1], None, None, 0) == 0
+            for i in range(5):
+                print(f"[paged graphs] replay {i}", flush=True)
+                set_lengths(i)
+                for k in range(6):  # each three times, in turn
+                    assert H.hipGraphLaunch(execs[k % 2], stream) == 0
+                assert H.hipStreamSynchronize(stream) == 0
+                for t, w in zip(outs, want[i]):
+                    assert np.array_equal(ctx.download_raw(t), w), i
+                for got, w in zip(eager(), want[i]):
+                    assert np.array_equal(got, w), i
+        finally:
+            for e in execs:
+                if e.value:
+                    H.hipGraphExecDestroy(e)
+            for g in graphs:
+                if g.value:
+                    H.hipGraphDestroy(g)
