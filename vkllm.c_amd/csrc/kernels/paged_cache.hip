@@ -18,8 +18,8 @@ namespace vk
 // arrive (none waits) takes the others' bits from the workspace, and has the prefix sums, the free list and the lengths in its
 // own LDS: it writes the lengths and the columns [keep, keep + need). The other workgroups write the remaining columns,
 // which hang on a row's own lengths only: the kept ids (unless in place) and NO_PAGE behind. One launch. Bound by latency
-// and by a CU's rate of LDS atomics: 256 rows of up to 512 pages of 65536 take 11.8 us, 16.8 with one marking workgroup;
-// 1000 rows of up to 700 of 400000 with slots and positions of 8000 tokens 33 us, 58 with five.
+// and by a CU's rate of LDS atomics: 256 rows of up to 512 pages of 65536 take 10.2 us, 16.8 with one marking workgroup; 1000
+// rows of up to 700 of 400000 with slots and positions of 8000 tokens 32 us.
 constexpr uint32_t kMaxTableThreads = 1024, kMinTableThreads = 256;
 
 struct PageTableArgs
@@ -34,7 +34,8 @@ struct PageTableArgs
     uint32_t *arrivals; // zero between launches
 };
 constexpr uint32_t kMarkColumns = 256; // columns of a row that a wave marks at once
-constexpr uint32_t kMarkPieces = 32, kMaxMarkers = 16;
+// 16 pieces: 16 rows of 700 columns 9.7 us for 8.8; 16 markers: 256 rows of 512 0.4 us more
+constexpr uint32_t kMarkPieces = 32, kMaxMarkers = 8;
 
 __device__ __forceinline__ uint32_t ceil_pages(uint32_t len, uint32_t R)
 {
@@ -161,10 +162,15 @@ __global__ __launch_bounds__(kMaxTableThreads) void page_table_kernel(PageTableA
             return;
         for (uint32_t w = t; w < words / 2; w += threads)
         {
-            uint64_t any = mine[w];
-#pragma unroll 8
-            for (uint32_t g = 0; g < a.markers; ++g)
-                any |= __hip_atomic_load(bits + (size_t)g * (words / 2) + w, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            uint64_t any = mine[w], theirs[kMaxMarkers];
+#pragma unroll
+            for (uint32_t g = 0; g < kMaxMarkers; ++g) // all on their way at once
+                theirs[g] = g < a.markers ? __hip_atomic_load(bits + (size_t)g * (words / 2) + w, __ATOMIC_RELAXED,
+                                                              __HIP_MEMORY_SCOPE_AGENT)
+                                          : 0;
+#pragma unroll
+            for (uint32_t g = 0; g < kMaxMarkers; ++g)
+                any |= theirs[g];
             ((uint64_t *)used)[w] = any;
         }
         __syncthreads();

@@ -65,20 +65,16 @@ __device__ __forceinline__ uint64_t read_lane(uint64_t v, uint32_t lane)
 // calls it; it starts and ends with the workgroup together.
 __device__ __forceinline__ uint64_t block_scan(uint64_t v, uint64_t *part, uint64_t &total)
 {
-    const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave, waves = blockDim.x / kWave;
+    const uint32_t lane = threadIdx.x & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const uint64_t s = wave_scan(v);
     __syncthreads();
     if (lane == kWave - 1)
         part[wave] = s;
     __syncthreads();
-    uint64_t before = 0;
-    total = 0;
-    for (int i = 0; i < waves; ++i)
-    {
-        before += i < wave ? part[i] : 0;
-        total += part[i];
-    }
-    return before + s - v;
+    // the waves' sums by the same scan: one after the other, 16 of them took 0.7 us
+    const uint64_t upto = wave_scan(lane < blockDim.x / kWave ? part[lane] : 0);
+    total = read_lane(upto, kWave - 1);
+    return (wave ? read_lane(upto, wave - 1) : 0) + s - v;
 }
 
 // the last b < n with start[b] <= k, for start[0] = 0 and sums that do not fall
