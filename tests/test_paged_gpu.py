@@ -438,3 +438,31 @@ def test_paged_attn_past_32_bit_offsets(ctx, vk):
     want[-1, :KV, R - 1], want[-1, KV:, R - 1] = k[0, 0], v[0, 0]
     want[1, :KV, 5], want[1, KV:, 5] = k[0, 2], v[0, 2]
     assert np.array_equal(got.view(np.uint16), want.view(np.uint16))
+
+
+def test_tables_and_lists_that_are_views(ctx, vk):
+    """A table in rows of a wider tensor, and lengths and counts that are columns of others: what lies beside them is not read."""
+    r = np.random.default_rng(31)
+    R, KV, H, hd = 16, 2, 4, 64
+    lengths = [70, 0, 33, 129, 1]
+    q, cache, table = make_attention(r, lengths, H, KV, hd, R, np.float16)
+    B, pages = len(lengths), cache.shape[0]
+    want = np.array([75, 17, 0, 129, 64])
+    counts = np.array([5, 17, 0, 1, 63])
+    with Bag(ctx) as bag:
+        def column(values):
+            return bag.view(values.astype(np.uint32).reshape(1, 1, 1, B), (0, 1, 3, 2), 6)
+
+        wide = bag.view(rows4(table), None, 7)
+        assert wide.contents.strides[2] == 4 * (table.shape[1] + 7) and column(want).contents.strides[3] == 28
+        out = bag.op("paged_attn", q.shape, vk.F16, vk.OP_PAGED_ATTN, [bag.put(q), bag.put(cache), wide],
+                     vk.PagedAttnParams(0.125, 1e4, True))
+        check_attention(ctx.download(out)[0], q, cache, table, 0.125, 1e4, True)
+        grown = bag.op("page_table", (1, 1, *table.shape), vk.U32, vk.OP_PAGE_TABLE, [column(want), wide],
+                       vk.PageTableParams(R, pages + 20))
+        new = ref.page_table(table, want, R, pages + 20)
+        assert np.array_equal(ctx.download(grown)[0, 0], new)
+        T = int(counts.sum())
+        slots = bag.op("slot_map", (1, 1, T, 2), vk.U32, vk.OP_SLOT_MAP,
+                       [bag.view(rows4(new), None, 3), column(want), column(counts)], vk.SlotMapParams(R))
+        assert np.array_equal(ctx.download(slots)[0, 0], ref.slot_map(new, want, counts, T, R))
