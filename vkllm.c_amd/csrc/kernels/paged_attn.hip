@@ -721,10 +721,15 @@ __global__ __launch_bounds__(256, HDP == 256 ? 1 : 2) void paged_attn_kernel(Pag
 #pragma unroll
                     for (uint32_t c = 0; c < kJoinFan; ++c)
                     {
-                        // a part without a largest score counts with 0, which keeps a sum that is not a number one
+                        // a part without a largest score counts with 0, which keeps a sum that is not a number one; a part
+                        // that is none not at all, whose sums may be infinite
                         const float f = ml[j][c].x == kNegInf ? 0.f : exp2_of(ml[j][c].x - x.m);
-                        x.l += f * ml[j][c].y;
-                        x.o += f * (f32x4){o[j][c][0].x, o[j][c][0].y, o[j][c][1].x, o[j][c][1].y};
+                        const f32x4 sums = {o[j][c][0].x, o[j][c][0].y, o[j][c][1].x, o[j][c][1].y};
+                        if (way + c * ways < size)
+                        {
+                            x.l += f * ml[j][c].y;
+                            x.o += f * sums;
+                        }
                     }
                     r[j] = x;
                 }
