@@ -9,7 +9,9 @@
  * out = sum_j softmax_j(scale * q . k_j) v_j, with q rotated to position length - 1 (unless rope_base is 0). Softmax and
  * sums are in 32 bits, and the result is rounded once. A row of length 0, and one whose every score is -inf, gives zeros;
  * lengths end at P * page_rows, and positions on pages that the cache does not have count as absent. Rows of the cache
- * past a sequence's end are never used, whatever they hold.
+ * past a sequence's end are never used, whatever they hold. Infinite and undefined numbers in those that are count as in the
+ * formula in 32 bits: a key whose score is -inf has no weight, a score of +inf or NaN leaves its head undefined, and an infinite
+ * value makes its dim infinite under any weight that is not 0 (undefined under 0, or with one of the other sign).
  * Partial results go through a workspace of the context, made by _init: captured into a hipGraph, the call is replayed on
  * the context's stream, and every tensor of it has been run once before (otherwise it is refused). */
 #ifndef VKLLM_OP_PAGED_ATTN_H

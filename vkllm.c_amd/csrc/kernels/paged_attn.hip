@@ -26,6 +26,7 @@
 namespace vk
 {
 
+typedef _Float16 half2 __attribute__((ext_vector_type(2)));
 typedef _Float16 half8 __attribute__((ext_vector_type(8)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 
@@ -99,7 +100,8 @@ template <bool F16, int HDP> struct PagedTile
     static constexpr int QP = HDP + (F16 ? 8 : 4);      // row pitch of the queries in LDS
     // rotated fp16 queries are kept as two fp16 parts of their halves (a rotation makes them up to sqrt(2) larger), and
     // probabilities as two parts, too: one part each cost 2^-12 on average in the result, as much as its own rounding does,
-    // and the matrix cores have the time
+    // and the matrix cores have the time. Of an infinite or undefined operand the first part's product alone counts: the
+    // second part may be 0 or of the other sign.
     static constexpr int QN = F16 ? 2 : 1;
     static constexpr int NP = kHeadsPerTile * HDP / 2 / 256; // query pairs that a thread stages
     // Workgroups per CU. fp16, us with 1 / 2 / 3: 50 rows of up to 8192 over 5 key heads of 128 56 / 58 / 64, 200 rows of up
@@ -118,6 +120,27 @@ __device__ __forceinline__ uint64_t quotient(uint64_t n, uint64_t d)
 __device__ __forceinline__ float exp2_of(float x)
 {
     return __builtin_amdgcn_exp2f(x);
+}
+
+// u's first part: 0 for 0 only, so that its product with an infinite key is infinite
+__device__ __forceinline__ _Float16 first_part(float u)
+{
+    const _Float16 h = (_Float16)u;
+    return h == (_Float16)0.f && u != 0.f ? (_Float16)copysignf(0x1p-24f, u) : h;
+}
+
+// both halves of a word within fp16's finite numbers, and what they are beyond them
+__device__ __forceinline__ uint32_t finite_halves(uint32_t w)
+{
+    const half2 most = {65504.f, 65504.f};
+    const half2 v = __builtin_elementwise_min(__builtin_elementwise_max(__builtin_bit_cast(half2, w), -most), most);
+    return __builtin_bit_cast(uint32_t, v);
+}
+__device__ __forceinline__ uint32_t beyond_halves(uint32_t w)
+{
+    const uint32_t v = finite_halves(w);
+    const half2 d = __builtin_bit_cast(half2, w) - __builtin_bit_cast(half2, v);
+    return __builtin_bit_cast(uint32_t, d);
 }
 
 // dynamic LDS, aligned for 16-byte accesses (left to chance, launches took 1 to 2 us more): lengths [B], queries
@@ -320,10 +343,11 @@ __global__ __launch_bounds__(256, HDP == 256 ? 1 : 2) void paged_attn_kernel(Pag
                     v = r.y * x + r.x * y;
                     if constexpr (F16)
                     {
-                        u *= 0.5f;
-                        v *= 0.5f;
-                        qs[(kHeadsPerTile + i) * QP + d0] = (T)(u - (float)(T)u);
-                        qs[(kHeadsPerTile + i) * QP + d1] = (T)(v - (float)(T)v);
+                        const float hu = 0.5f * u, hv = 0.5f * v;
+                        u = (float)first_part(hu);
+                        v = (float)first_part(hv);
+                        qs[(kHeadsPerTile + i) * QP + d0] = (T)(hu - u);
+                        qs[(kHeadsPerTile + i) * QP + d1] = (T)(hv - v);
                     }
                 }
                 qs[i * QP + d0] = (T)u;
@@ -420,10 +444,10 @@ __global__ __launch_bounds__(256, HDP == 256 ? 1 : 2) void paged_attn_kernel(Pag
         auto query = [&](int n, int s) {
             return *(const u32x4 *)(qs + q_at + n * kHeadsPerTile * QP + (F16 ? 32 : 16) * s);
         };
-        f32x4 x[NT];
+        f32x4 x[NT], rest[NT]; // scores; what the queries' second parts add
 #pragma unroll
         for (int i = 0; i < NT; ++i)
-            x[i] = (f32x4){0.f, 0.f, 0.f, 0.f};
+            x[i] = rest[i] = (f32x4){0.f, 0.f, 0.f, 0.f};
         if constexpr (!FULL)
 #pragma unroll
             for (int k = 0; k < KS; ++k)
@@ -433,7 +457,7 @@ __global__ __launch_bounds__(256, HDP == 256 ? 1 : 2) void paged_attn_kernel(Pag
                         kr[i][k] = (u32x4){0, 0, 0, 0};
         if constexpr (F16)
         {
-            auto score = [&](int n) {
+            auto score = [&](int n, f32x4(&x)[NT]) {
 #pragma unroll
                 for (int k = 0; k < KS; ++k)
                 {
@@ -443,9 +467,9 @@ __global__ __launch_bounds__(256, HDP == 256 ? 1 : 2) void paged_attn_kernel(Pag
                         x[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8, kr[i][k]), q, x[i], 0, 0, 0);
                 }
             };
-            score(0);
+            score(0, x);
             if (a.rope.style)
-                score(1);
+                score(1, rest);
         }
         else
         {
@@ -481,6 +505,8 @@ __global__ __launch_bounds__(256, HDP == 256 ? 1 : 2) void paged_attn_kernel(Pag
 #pragma unroll
             for (int r = 0; r < 4; ++r)
             {
+                if constexpr (F16) // where a score is finite, so is the rest
+                    x[i][r] += fabsf(rest[i][r]) < INFINITY ? rest[i][r] : 0.f;
                 x[i][r] *= a.scale_log2;
                 if (!whole && 4 * g + r >= n[i])
                     x[i][r] = kNegInf;
@@ -527,15 +553,50 @@ __global__ __launch_bounds__(256, HDP == 256 ? 1 : 2) void paged_attn_kernel(Pag
                 p[j] = (_Float16)x[j / 4][j % 4];
                 q[j] = (_Float16)(x[j / 4][j % 4] - (float)p[j]);
             }
-#pragma unroll
-            for (int d = 0; d < VD; ++d)
-            {
-                u32x4 v; // 8 keys of dim VD * c + d
+            auto values = [&](int d) { // 8 keys of dim VD * c + d
+                u32x4 v;
 #pragma unroll
                 for (int j = 0; j < 4; ++j)
                     v[j] = __builtin_amdgcn_perm(vr[2 * j + 1][d / 2], vr[2 * j][d / 2], d % 2 ? 0x07060302u : 0x05040100u);
-                o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8, v), p, o[d], 0, 0, 0);
-                o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8, v), q, o[d], 0, 0, 0);
+                return v;
+            };
+            // the values times 0: not a number if one of them is none or infinite. One row of 12000 positions, 32 heads on 8: 18.3
+            // us for 18.0 without; batches and long rows level.
+            float sum = 0.f;
+#pragma unroll
+            for (int j = 0; j < 2 * 4; ++j)
+#pragma unroll
+                for (int w = 0; w < VW; ++w)
+                    sum = __builtin_amdgcn_fdot2(__builtin_bit_cast(half2, vr[j][w]), (half2){0.f, 0.f}, sum, false);
+            if (__builtin_expect(__any(sum != sum), 0))
+            {
+                // What values are beyond the finite numbers (infinite, undefined; 0 for the others) counts once for every
+                // weight that is not 0; the rest of them goes the way of all values.
+                half8 one;
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                    one[j] = x[j / 4][j % 4] > 0.f ? (_Float16)1.f : p[j];
+#pragma unroll
+                for (int d = 0; d < VD; ++d)
+                {
+                    u32x4 v = values(d);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        v[j] = beyond_halves(v[j]);
+                    o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8, v), one, o[d], 0, 0, 0);
+                }
+#pragma unroll
+                for (int j = 0; j < 2 * 4; ++j)
+#pragma unroll
+                    for (int w = 0; w < VW; ++w)
+                        vr[j][w] = finite_halves(vr[j][w]);
+            }
+#pragma unroll
+            for (int d = 0; d < VD; ++d)
+            {
+                const half8 v = __builtin_bit_cast(half8, values(d));
+                o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, p, o[d], 0, 0, 0);
+                o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, q, o[d], 0, 0, 0);
             }
         }
         else
