@@ -1,0 +1,47 @@
+"""Edges of the operators of batched generation: sources that no call has written yet under stream capture."""
+import ctypes
+
+import numpy as np
+import pytest
+
+from test_paged_gpu import Bag, rows4
+from test_zz_no_alloc import _hip_runtime
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("which", ["history", "rules", "mask"])
+def test_adjust_logits_of_a_source_that_never_ran_is_refused_under_capture(ctx, vk, which):
+    """History, rules or mask that an operator has yet to write have no memory: the call under capture is refused, makes
+    none, though the context has a free piece of that size, and leaves the capture as it was."""
+    print(f"[capture] {which}", flush=True)
+    H, L = _hip_runtime(), vk.lib()
+    stream, graph = ctypes.c_void_p(), ctypes.c_void_p()
+    vk.check("stream", L.vkllm_hip_context_stream(ctx.vp, ctypes.byref(stream)))
+    B, V, width = 2, 100, {"history": 9, "rules": 6, "mask": 4}[which]
+    with Bag(ctx) as bag:
+        x = bag.put(np.linspace(-3, 3, B * V).reshape(1, 1, B, V).astype(np.float16))
+        rules = np.zeros((B, 4), np.uint32)
+        rules[:, 0] = np.float32(1).view(np.uint32)
+        srcs = {"history": None, "rules": bag.put(rows4(rules)), "mask": None}
+        never = ctx.tensor([1, 1, B, width], vk.U32, op=vk.OP_PAGE_TABLE, srcs=[bag.put(rows4(np.zeros((1, B))))],
+                           params=vk.PageTableParams(16, 4))
+        srcs[which] = never
+        y = ctx.tensor([1, 1, B, V], vk.F16, op=vk.OP_ADJUST_LOGITS, srcs=[x, *srcs.values()])
+        bag.made += [never, y]
+        ctx.upload(y, np.zeros((1, 1, B, V), np.float16))
+        ctx.free(ctx.tensor([1, 1, B, width], vk.U32))
+        assert not never.contents.data.dev
+        assert H.hipStreamBeginCapture(stream, 0) == 0
+        rc = L.vkllm_op_adjust_logits_run(ctx.vp, ctx.cmds, y)
+        end = H.hipStreamEndCapture(stream, ctypes.byref(graph))
+        if graph.value:
+            H.hipGraphDestroy(graph)
+        assert rc == vk.ERR_ARGS and end == 0 and not never.contents.data.dev
+        first = np.zeros((B, width), np.uint32)
+        if which == "rules":
+            first[:, 0] = np.float32(1).view(np.uint32)
+        ctx.upload(never, rows4(first))
+        vk.check("adjust_logits", ctx.run_op("adjust_logits", y))
+        got = ctx.download(y)
+        assert np.isneginf(got).all() if which == "mask" else np.array_equal(got, ctx.download(x))

@@ -393,21 +393,20 @@ extern "C" vkllm_err_t vkllm_op_adjust_logits_run(struct vkllm_context *context,
 {
     DeviceScope device_scope(context);
     _CHECK(vkllm_op_adjust_logits_init(context, commands, tensor));
+    for (vkllm_tensor *src : tensor->srcs)
+        if (src)
+            CHECK_VIEW(src);
+    CHECK_VIEW(tensor);
+    _CHECK(node_memory(context, tensor)); // before any view is made: that gives a source memory
     vk::WordRows rows[3] = {};
-    for (int i = 0; i < 4; ++i)
+    for (int i = 1; i < 4; ++i)
     {
         if (!tensor->srcs[i])
             continue;
-        CHECK_VIEW(tensor->srcs[i]);
-        if (i > 0)
-        {
-            vk::TView w = tview(context, tensor->srcs[i]);
-            NEED_DEV(w);
-            rows[i - 1] = {(const uint32_t *)w.p, w.s[2], w.n[3]};
-        }
+        vk::TView w = tview(context, tensor->srcs[i]);
+        NEED_DEV(w);
+        rows[i - 1] = {(const uint32_t *)w.p, w.s[2], w.n[3]};
     }
-    CHECK_VIEW(tensor);
-    _CHECK(node_memory(context, tensor));
     vk::TView x = tview(context, tensor->srcs[0]), out = tview(context, tensor);
     NEED_DEV(x);
     NEED_DEV(out);
