@@ -1,10 +1,12 @@
-"""Edges of the operators of batched generation: sources that no call has written yet under stream capture."""
+"""Edges of the operators of batched generation: sources that no call has written yet under stream capture, a table in place
+whose first columns hold anything."""
 import ctypes
 
 import numpy as np
 import pytest
 
-from test_paged_gpu import Bag, rows4
+import paged_ref as ref
+from test_paged_gpu import Bag, rows4, table_step
 from test_zz_no_alloc import _hip_runtime
 
 pytestmark = pytest.mark.gpu
@@ -45,3 +47,21 @@ def test_adjust_logits_of_a_source_that_never_ran_is_refused_under_capture(ctx, 
         vk.check("adjust_logits", ctx.run_op("adjust_logits", y))
         got = ctx.download(y)
         assert np.isneginf(got).all() if which == "mask" else np.array_equal(got, ctx.download(x))
+
+
+@pytest.mark.parametrize("B,P,R,pages", [(1, 3, 16, 9), (5, 7, 16, 40), (70, 300, 4, 9000), (300, 600, 16, 70000)])
+def test_page_table_in_place_over_anything(ctx, vk, B, P, R, pages):
+    """A table in place needs no more of its first contents than a length of 0 in every row: whatever the columns hold, the
+    first step leaves the pages of the rows that grew and nothing behind them, also in rows whose wanted length is over the
+    table's width, and in those that do not fit."""
+    print(f"[page_table] B={B} P={P} R={R} pages={pages}", flush=True)
+    r = np.random.default_rng(B)
+    old = r.integers(0, 1 << 32, (B, 1 + P), dtype=np.uint32)
+    old[:, 1:][r.random((B, P)) < 0.5] = r.integers(0, pages)
+    old[:, 0] = 0
+    want = r.integers(0, P * R + 1, B)
+    want[r.random(B) < 0.4] = P * R + 1 + r.integers(0, 1000)
+    want[0] = P * R + 1
+    for in_place in (True, False):
+        got = table_step(ctx, vk, old, want, R, pages, in_place)
+        assert np.array_equal(got, ref.page_table(old, want, R, pages)), in_place

@@ -68,7 +68,10 @@ __global__ __launch_bounds__(kMaxTableThreads) void page_table_kernel(PageTableA
             uint32_t *to = a.out.p + (size_t)b * a.out.stride + 1;
             if (!a.old)
             {
-                for (uint32_t c = (want > (uint64_t)P * R ? P : ceil_pages(want, R)) + t; c < P; c += threads)
+                // A wanted length over the row's width leaves the row as it is. Its own length may just be rewritten, cut to
+                // the width: either way it is as many pages.
+                const uint32_t kept = want > (uint64_t)P * R ? row_pages(to[-1], want, R, P).keep : ceil_pages(want, R);
+                for (uint32_t c = kept + t; c < P; c += threads)
                     to[c] = kNoPage;
                 continue;
             }
