@@ -1,5 +1,5 @@
 """Edges of the operators of batched generation: sources that no call has written yet under stream capture, a table in place
-whose first columns hold anything."""
+whose first columns hold anything, penalties by quotients of any size."""
 import ctypes
 
 import numpy as np
@@ -65,3 +65,25 @@ def test_page_table_in_place_over_anything(ctx, vk, B, P, R, pages):
     for in_place in (True, False):
         got = table_step(ctx, vk, old, want, R, pages, in_place)
         assert np.array_equal(got, ref.page_table(old, want, R, pages)), in_place
+
+
+@pytest.mark.parametrize("dtype", [np.float16, np.float32])
+@pytest.mark.parametrize("rep", [1.1, 1.3, 3.0, 1e-39, 2e-42, 3e38, 1.0 / 3.0], ids=str)
+def test_penalties_are_quotients(ctx, vk, rep, dtype):
+    """x / repetition and x * repetition as 32 bits round them, once (and once more to 16): also where 1 / repetition is no
+    number of 32 bits."""
+    print(f"[adjust_logits] repetition {rep} {dtype.__name__}", flush=True)
+    B, V = 3, 4099
+    r = np.random.default_rng(11)
+    x = (r.standard_normal((1, 1, B, V)) * np.exp(r.uniform(-12, 4, (1, 1, B, V)))).astype(dtype)
+    history = np.concatenate((np.full((B, 1), V), np.tile(np.arange(V), (B, 1))), 1)
+    rules = np.zeros((B, 4), np.uint32)
+    rules[:, 0] = np.float32(rep).view(np.uint32)
+    with Bag(ctx) as bag:
+        t = bag.op("adjust_logits", x.shape, vk.F16 if dtype == np.float16 else vk.F32, vk.OP_ADJUST_LOGITS,
+                   [bag.put(x), bag.put(rows4(history)), bag.put(rows4(rules))])
+        got = ctx.download(t)
+    x32 = x.astype(np.float32)
+    with np.errstate(over="ignore", under="ignore"):
+        want = np.where(x32 > 0, x32 / np.float32(rep), x32 * np.float32(rep)).astype(dtype)
+    assert np.array_equal(got, want)
