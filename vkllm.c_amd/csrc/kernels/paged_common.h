@@ -27,13 +27,15 @@ __device__ __forceinline__ uint32_t scalar_word(const uint32_t *p)
 }
 
 // (cos, sin) of position * turns full turns. The product is in 64 bits and only its fraction goes on: at position 10^5
-// a 32-bit angle would be off by 2^-8.
+// a 32-bit angle would be off by 2^-8. What the fraction's 32 bits leave out turns the result a little further, by less than
+// 2 pi 2^-26, which is its own sine; without it fp32 rows are 1.4 times as far off as their arithmetic makes them, 1.07 with it.
 __device__ __forceinline__ float2 turn_at(uint32_t position, double turns)
 {
-    const double full = (double)position * turns;
-    float2 r;
-    sincospif(2.0f * (float)(full - rint(full)), &r.y, &r.x);
-    return r;
+    const double full = (double)position * turns, part = full - rint(full);
+    const float near = (float)part, rest = 6.283185307f * (float)(part - (double)near);
+    float s, c;
+    sincospif(2.0f * near, &s, &c);
+    return {fmaf(-s, rest, c), fmaf(c, rest, s)};
 }
 
 template <int ctrl, int row_mask> __device__ __forceinline__ uint64_t dpp_add64(uint64_t v)
