@@ -43,7 +43,7 @@ template <typename T, bool WIDE> __global__ __launch_bounds__(1024) void adjust_
     constexpr uint32_t N = 16 / sizeof(T), VECS = 2;
     typedef T TN __attribute__((ext_vector_type(N)));
     typedef Logits<T, N> Vec;
-    extern __shared__ uint32_t lds[];
+    extern __shared__ __align__(16) uint32_t lds[]; // also read as 16-byte vectors
     __shared__ float values[kBiasesInLds]; // the first biases' values
     const uint32_t t = threadIdx.x, threads = blockDim.x, b = blockIdx.y, V = a.x.n[3], tile = a.tile;
     uint32_t *count = lds, *last = WIDE ? lds + tile : lds;

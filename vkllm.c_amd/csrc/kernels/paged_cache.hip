@@ -57,7 +57,7 @@ __device__ __forceinline__ RowPages row_pages(uint32_t had, uint32_t want, uint3
 
 __global__ __launch_bounds__(kMaxTableThreads) void page_table_kernel(PageTableArgs a)
 {
-    extern __shared__ uint32_t lds[];
+    extern __shared__ __align__(16) uint32_t lds[]; // also read as 64-bit words
     const uint32_t t = threadIdx.x, threads = blockDim.x, B = a.out.B, P = a.out.P, R = a.R;
     if (blockIdx.x >= a.markers)
     {
