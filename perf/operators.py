@@ -11,7 +11,8 @@ then NONE. Four kinds of case:
   logits   ADJUST_LOGITS: repetition, frequency and presence penalties, token biases and a grammar's mask
 
 With `own` false, run() computes them in elementary torch operations in 32 bits (angles in 64); with it true it calls
-the VKLLM_OP_* operators on a context's stream.
+the VKLLM_OP_* operators on a context's stream, which is torch's current stream from the first prepare() on: what a caller
+does with the results in torch comes after them.
 """
 import ctypes
 import math
@@ -227,6 +228,10 @@ class Program:
         V = self.V = framework()
         if Program.context is None:
             Program.context = V.Ctx(0)
+            stream = ctypes.c_void_p()
+            V.check("stream", V.lib().vkllm_hip_context_stream(Program.context.vp, ctypes.byref(stream)))
+            torch.cuda.synchronize()  # what torch has done so far was on another stream
+            torch.cuda.set_stream(torch.cuda.ExternalStream(stream.value))
         self.ctx, self.L, self.tensors, self.todo, self.seen = Program.context, V.lib(), [], [], None
         F = {"f16": V.F16, "f32": V.F32}.get(case.get("dtype"))
         page, kind = case.get("page"), case["kind"]
