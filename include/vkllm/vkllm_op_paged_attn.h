@@ -5,7 +5,8 @@
  * [pages, 2 * KV, page_rows, head_dim], packed, page_rows a multiple of 16, H a multiple of KV: query head h reads key
  * head h / (H / KV)), all fp16 or all fp32; srcs[2] is the page table (VKLLM_OP_PAGE_TABLE, uint32 [1, 1, B, 1 + P], B <= 4096).
  * P * page_rows is at most 2^31.
- * Row b is the last token of its sequence, whose keys and values the cache holds already: over positions j < length
+ * Row b is the last token of its sequence (one token a row: the tokens of a prompt do not attend through this operator), whose
+ * keys and values the cache holds already: over positions j < length
  * out = sum_j softmax_j(scale * q . k_j) v_j, with q rotated to position length - 1 (unless rope_base is 0). Softmax and
  * sums are in 32 bits, and the result is rounded once. A row of length 0, and one whose every score is -inf, gives zeros;
  * lengths end at P * page_rows, and positions on pages that the cache does not have count as absent. Rows of the cache
