@@ -1,5 +1,5 @@
 """Edges of the operators of batched generation: sources that no call has written yet under stream capture, a table in place
-whose first columns hold anything, penalties by quotients of any size, rotations as near as 32 bits allow."""
+whose first columns hold anything, penalties by quotients of any size, rotations as near as 32 bits allow, rows without a token."""
 import ctypes
 
 import numpy as np
@@ -115,3 +115,16 @@ def test_rotations_in_32_bits(ctx, vk, neox):
     rms = lambda e: float(np.sqrt((e.astype(np.float64) ** 2).mean()))  # noqa: E731
     print(f"  {rms(got - want):.3e}, nearest cosines and sines {rms(near - want):.3e}", flush=True)
     assert rms(got - want) <= 1.2 * rms(near - want)
+
+
+def test_a_token_in_every_row(ctx, vk):
+    """With counts of 1 in all rows token b is row b's, whichever rows have no sequence; those get no slot. With counts of 0 there
+    the tokens behind move up."""
+    table = np.array([[20, 4, 9], [0, NONE, NONE], [3, 7, NONE], [0, NONE, NONE], [16, 2, NONE]], np.uint32)
+    lengths = table[:, 0]
+    for counts, want in ((np.ones(5), [[9 * 16 + 3, 19], [NONE, 0], [7 * 16 + 2, 2], [NONE, 0], [2 * 16 + 15, 15]]),
+                         (lengths > 0, [[9 * 16 + 3, 19], [7 * 16 + 2, 2], [2 * 16 + 15, 15], [NONE, 0], [NONE, 0]])):
+        with Bag(ctx) as bag:
+            t = bag.op("slot_map", (1, 1, 5, 2), vk.U32, vk.OP_SLOT_MAP,
+                       [bag.put(rows4(table)), bag.put(rows4(lengths[None])), bag.put(rows4(counts[None]))], vk.SlotMapParams(16))
+            assert ctx.download(t)[0, 0].tolist() == want
