@@ -11,6 +11,8 @@ from test_zz_no_alloc import _hip_runtime
 
 pytestmark = pytest.mark.gpu
 
+NONE = ref.NONE
+
 
 @pytest.mark.parametrize("which", ["history", "rules", "mask"])
 def test_adjust_logits_of_a_source_that_never_ran_is_refused_under_capture(ctx, vk, which):
