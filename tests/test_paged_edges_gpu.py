@@ -1,12 +1,13 @@
 """Edges of the operators of batched generation: sources that no call has written yet under stream capture, a table in place
-whose first columns hold anything, penalties by quotients of any size, rotations as near as 32 bits allow, rows without a token."""
+whose first columns hold anything, penalties by quotients of any size, rotations as near as 32 bits allow, rows without a token,
+and how many (sequence, key head) pairs share the GPU."""
 import ctypes
 
 import numpy as np
 import pytest
 
 import paged_ref as ref
-from test_paged_gpu import Bag, rows4, table_step
+from test_paged_gpu import Bag, check_attention, make_attention, rows4, run_attention, table_step
 from test_zz_no_alloc import _hip_runtime
 
 pytestmark = pytest.mark.gpu
@@ -130,3 +131,15 @@ def test_a_token_in_every_row(ctx, vk):
             t = bag.op("slot_map", (1, 1, 5, 2), vk.U32, vk.OP_SLOT_MAP,
                        [bag.put(rows4(table)), bag.put(rows4(lengths[None])), bag.put(rows4(counts[None]))], vk.SlotMapParams(16))
             assert ctx.download(t)[0, 0].tolist() == want
+
+
+@pytest.mark.parametrize("dtype", [np.float16, np.float32])
+@pytest.mark.parametrize("lengths,H,KV", [([8200], 8, 8), ([6400], 10, 10), ([6300], 11, 11), ([5600], 48, 12), ([3000, 2900], 24, 6),
+                                          ([5600], 96, 12), ([2900], 120, 24), ([2800], 130, 26), ([2700, 0, 2600], 65, 13)],
+                         ids=lambda v: str(v))
+def test_rows_on_one_workgroup_a_cu(ctx, vk, lengths, H, KV, dtype):
+    """Numbers of (sequence, key head) pairs at both sides of where rows of 128 dims go to half of the workgroups."""
+    print(f"[paged_attn] {lengths} {H} {KV} {dtype.__name__}", flush=True)
+    q, cache, table = make_attention(np.random.default_rng(H + KV), lengths, H, KV, 128, 16, dtype)
+    got = run_attention(ctx, vk, q, cache, table, 128 ** -0.5, 1e4, True)
+    check_attention(got, q, cache, table, 128 ** -0.5, 1e4, True)

@@ -198,10 +198,16 @@ __global__ __launch_bounds__(256, HDP == 256 ? 1 : 2) void paged_attn_kernel(Pag
         // the second one's loads meanwhile; few units of few rows would have fewer loads on their way, for the same joins.
         // us with all / half of them: 2 rows of up to 131072 on 4 key heads 76.7 / 71, 1 of 3000 on 32 16.1 / 14.2, 2 of 1100
         // 18.3 / 13, 50 ragged ones of up to 8192 on 5 58 / 56, and fp32 60 / 58.5; but 64 of 8192 on 8 358 / 360 (fp32, of 768,
-        // 72 / 74), and kept out 1 of 12000 on 8 18.5 / 20.6, 2048 of 100 196 / 216, 64 of 1024 on 8 of 64 dims 27 / 36.
+        // 72 / 74), and kept out 2048 of 100 196 / 216, 64 of 1024 on 8 of 64 dims 27 / 36.
+        // With 1 to 4 units a workgroup the gain hangs on how many (sequence, key head)s are cut, and on how large their parts
+        // are. 8 totals between 530 and 2000 units, half of the workgroups against all, in the mean (and from, to): 2 and 4 query
+        // heads to a key head, 4 pairs +1% (-17, +13), 8 -1% (-12, +12), 12 -10% (-26, +1), 16 -5% (-12, +5), 32 -9% (-21, +1); 5 to
+        // 16 query heads, 8 +1% (-8, +21), 12 -8% (-32, +4), 16 +2% (-11, +24), 20 -3% (-35, +25), 24 +4% (-11, +23), 26 -9% (-40,
+        // +1), 28 -14%, 32 -14%. So from between 8 and 12 pairs where parts are small, else from between 24 and 26.
         const uint64_t units = (total & ((1ull << 40) - 1)) * heads, rows = (total >> 40) * heads;
         const uint32_t n = gridDim.x;
-        const bool alone = FULL && HDP == 128 && units >= 6 * rows && (units >= 4 * n || (units > n && 16 * rows >= n));
+        const bool alone = FULL && HDP == 128 && units >= 6 * rows &&
+                           (units >= 4 * n || (units > n && (a.tile_heads <= 4 ? 48 : 20) * rows >= n));
         const uint32_t sharers = alone ? (n + 1) / 2 : n;
         extra = units > 4 * n ? kSegmentUnits : 0;
         share = quotient(weigh(total) + sharers - 1, sharers);
