@@ -3,7 +3,8 @@
 // For a sequence and a key head, with its queries q_h (up to 16 heads that share the key head), keys k_j and values v_j:
 //   out_h = sum_j p_hj v_j / sum_j p_hj,  p_hj = 2^(log2(e) * scale * q_h . k_j - m_h)
 // for any m_h, in one pass over the cache: m_h follows the largest score, and sums formed before it rose are scaled down.
-// Every byte of keys and values is read once and used for 2 operations per query head, so HBM bounds it.
+// Every byte of keys and values is read once per tile of 16 query heads and used for 2 operations per query head, so HBM
+// bounds it.
 //
 // Work is split without knowing the lengths on the host: a unit is KT consecutive positions of one (sequence, key head),
 // all units of the batch are numbered in that order, and each of a fixed number of workgroups (as many as are resident)
@@ -76,7 +77,7 @@ __device__ __forceinline__ float2 get2(const float *p)
 
 // A thread joins kJoinFan parts of four dims (of eight, loads of both on their way, where a part has more than 256 fours).
 // Where it has 128 or fewer, 2, 4 or 8 lanes share a four, so a level takes up to 64 parts. One row of 2000 positions, us
-// against pairs of dims joined through LDS: 16 heads on 1 key head 14.8 for 27, 32 on 8 9.5 for 13.1. 16 parts a thread
+// against pairs of dims joined through LDS: 16 heads on 1 key head 15.0 for 27, 32 on 8 9.6 for 13.1. 16 parts a thread
 // took 0.5 to 2 us more nearly everywhere: a level's cost is the round trip and the code's way to the CU.
 constexpr uint32_t kJoinFan = 8, kJoinLevels = 4;
 static_assert(1u << 3 * kJoinLevels >= kPagedMaxWorkgroups && kPagedArrivals == 2 * kJoinLevels * kPagedMaxWorkgroups);

@@ -15,11 +15,11 @@ namespace vk
 // the number of free pages keep what they had.
 //
 // The first `markers` workgroups mark the kept pages, each those of its share of the rows, in bits in LDS. The last of them to
-// arrive (none waits) takes the others' bits from the workspace, and has the prefix sums, the free list and the lengths in its
-// own LDS: it writes the lengths and the columns [keep, keep + need). The other workgroups write the remaining columns,
+// arrive (none waits) takes the others' bits from the workspace, and has the prefix sums, the free pages' ranks and the lengths
+// in its own LDS: it writes the lengths and the columns [keep, keep + need). The other workgroups write the remaining columns,
 // which hang on a row's own lengths only: the kept ids (unless in place) and NO_PAGE behind. One launch. Bound by latency
 // and by a CU's rate of LDS atomics: 256 rows of up to 512 pages of 65536 take 10.2 us, 16.8 with one marking workgroup; 1000
-// rows of up to 700 of 400000 with slots and positions of 8000 tokens 32 us.
+// rows of up to 700 of 400000 26.5 us, in place 27; a step that hands out 20000 pages 56.
 constexpr uint32_t kMaxTableThreads = 1024, kMinTableThreads = 256;
 
 struct PageTableArgs
@@ -34,7 +34,9 @@ struct PageTableArgs
     uint32_t *arrivals; // zero between launches
 };
 constexpr uint32_t kMarkColumns = 256; // columns of a row that a wave marks at once
-// 16 pieces: 16 rows of 700 columns 9.7 us for 8.8; 16 markers: 256 rows of 512 0.4 us more
+// 16 pieces: 16 rows of 700 columns 9.7 us for 8.8. us with up to 4 / 8 / 16 / 32 markers: 256 rows of 512 11.0 / 9.8 / 10.2 / 10.4,
+// 256 of 2048 23.2 / 18.4 / 17.7 / 22.0, 1000 of 700 32.7 / 26.6 / 27.0 / 28.8, 30 of 8192 14.5 / 12.0 / 11.7 / 13.7; only many
+// narrow rows want more: 4000 of 64 38.1 / 26.3 / 21.5 / 21.9.
 constexpr uint32_t kMarkPieces = 32, kMaxMarkers = 8;
 
 __device__ __forceinline__ uint32_t ceil_pages(uint32_t len, uint32_t R)
