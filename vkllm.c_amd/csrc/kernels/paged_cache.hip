@@ -19,7 +19,7 @@ namespace vk
 // in its own LDS: it writes the lengths and the columns [keep, keep + need). The other workgroups write the remaining columns,
 // which hang on a row's own lengths only: the kept ids (unless in place) and NO_PAGE behind. One launch. Bound by latency
 // and by a CU's rate of LDS atomics: 256 rows of up to 512 pages of 65536 take 10.2 us, 16.8 with one marking workgroup; 1000
-// rows of up to 700 of 400000 26.5 us, in place 27; a step that hands out 20000 pages 56.
+// rows of up to 700 of 400000 26.5 us, in place 27; a step that hands out 14000 pages 56.
 constexpr uint32_t kMaxTableThreads = 1024, kMinTableThreads = 256;
 
 struct PageTableArgs
