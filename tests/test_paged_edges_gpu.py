@@ -143,3 +143,35 @@ def test_rows_on_one_workgroup_a_cu(ctx, vk, lengths, H, KV, dtype):
     q, cache, table = make_attention(np.random.default_rng(H + KV), lengths, H, KV, 128, 16, dtype)
     got = run_attention(ctx, vk, q, cache, table, 128 ** -0.5, 1e4, True)
     check_attention(got, q, cache, table, 128 ** -0.5, 1e4, True)
+
+
+def test_page_table_of_the_most_rows_and_pages(ctx, vk):
+    """4096 rows and 524288 pages at once: the most that the kernel's LDS is asked for."""
+    B, P, R, pages = 4096, 150, 16, 524288
+    print(f"[page_table] B={B} P={P} pages={pages}", flush=True)
+    r = np.random.default_rng(3)
+    table = np.full((B, 1 + P), NONE, np.uint32)
+    table[:, 0] = r.integers(0, P * R + 1, B)
+    order, at = r.permutation(pages), 0
+    for b in range(B):
+        n = -(-int(table[b, 0]) // R)
+        table[b, 1:1 + n] = order[at:at + n]
+        at += n
+    want = np.where(r.random(B) < 0.5, r.integers(0, P * R + 1, B), table[:, 0] + 1)
+    want[7], want[8] = P * R + 5, 0
+    new = ref.page_table(table, want, R, pages)
+    for in_place in (False, True):
+        assert np.array_equal(table_step(ctx, vk, table, want, R, pages, in_place), new), in_place
+
+
+@pytest.mark.parametrize("dtype", [np.float16, np.float32])
+def test_paged_attn_of_the_most_rows_and_heads(ctx, vk, dtype):
+    """4096 rows of 16 heads of 256 dims on one key head: the most that the kernel's LDS is asked for."""
+    print(f"[paged_attn] 4096 rows {dtype.__name__}", flush=True)
+    r = np.random.default_rng(4)
+    lengths = np.where(r.random(4096) < 0.9, 0, r.integers(1, 40, 4096))
+    lengths[-1] = 300
+    q, cache, table = make_attention(r, lengths.tolist(), 16, 1, 256, 16, dtype)
+    got = run_attention(ctx, vk, q, cache, table, 1 / 16, 1e4, False)
+    check_attention(got, q, cache, table, 1 / 16, 1e4, False)
+    assert not got[lengths == 0].any()
